@@ -405,6 +405,51 @@ int mscl_sgd_step_dev(float* p, const float* g, float* buf, uint16_t* p_bf16, in
                       float max_norm, const float* lr_dev, float momentum, float wd, void* stream);
 int mscl_cast_bf16(const float* src, uint16_t* dst, int64_t n, void* stream);
 
+/* ---- AdamW over many tensors, moments in 32 or in 8 bits (adamw.hip) --------------------------------------------------------
+ * torch.optim.AdamW (decoupled decay, amsgrad off), which mmcv's build_optimizer wires for `optimizer=dict(type='AdamW', ...)`
+ * (mmaction/apis/train.py:94), with clip_grad_norm_ over all tensors ahead of it (mmcv OptimizerHook, apis/train.py:111-119) and the
+ * per-parameter multipliers of `paramwise_cfg`.  Two launches whatever the number of tensors.
+ *   step t = ++words.step;  c = min(1, max_norm / (|g| + 1e-6)) (1 when max_norm <= 0), *grad_norm = |g| before the clip;
+ *   m = b1 m + (1-b1) c g;  v = b2 v + (1-b2) (c g)^2;
+ *   p = p (1 - lr lr_mult decay) - lr lr_mult / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps);  shadow = round(p)
+ * Bit-reproducible (no atomics).  A non-finite gradient behaves as in torch: it goes into m, v and p.
+ * States: flat buffers in which tensor i starts at element `off`, a multiple of MSCL_ADAMW_BLOCK, and is padded with zeros to a whole
+ * number of blocks.  8 bits: one byte per element and moment plus, per block and moment, one exponent byte E (fp32's bias; 255: the
+ * block holds a non-finite value and reads as NaN).  m: sign, 4-bit exponent field e, 3-bit mantissa k, value (1 + k/8) 2^(E-127 + e-15)
+ * for e > 0, k/8 2^(E-127-14) for e = 0.  v: 5-bit e, value (1 + k/8) 2^(E-127 + e-31), k/8 2^(E-127-30) for e = 0.  Rounded up or
+ * down at random, without bias, by a hash of (seed, t, element); p uses the moments before they are rounded. */
+#define MSCL_NONE 0
+#define MSCL_F32  1
+#define MSCL_BF16 2
+#define MSCL_F16  3
+#define MSCL_ADAMW_BLOCK 256       /* elements that share an exponent; alignment of a tensor inside the state buffers */
+#define MSCL_ADAMW_CHUNK 4096      /* elements per entry of chunk_tensor (the last chunk of a tensor may be short) */
+#define MSCL_ADAMW_PARTS 256       /* doubles in `partials` */
+#define MSCL_ADAMW_WORDS 32        /* bytes in `words`: int64 step, 8 bytes derived from it, uint32 derived, uint32 seed at byte 20 */
+typedef struct {
+  float* p;                 /* fp32 parameter, n elements */
+  uint16_t* shadow;         /* 16-bit copy to refresh, or NULL when shadow_type is MSCL_NONE */
+  int64_t n, off;           /* elements; first element in the state buffers */
+  float lr_mult, decay;     /* decay: weight_decay times the tensor's multiplier */
+  int32_t first_chunk;      /* index of its first chunk */
+  int32_t pad;
+} mscl_adamw_tensor;
+typedef struct {
+  const mscl_adamw_tensor* tensors;      /* device */
+  const void* const* grads;              /* device: one pointer per tensor */
+  const int32_t* chunk_tensor;           /* device: n_chunks tensor indices, ascending */
+  void* m; void* v;                      /* float or uint8_t, 16-byte aligned */
+  uint8_t* exponents;                    /* 8 bits: [2][n_blocks] */
+  int64_t n_blocks;
+  void* words; double* partials; float* grad_norm; const float* lr;     /* device */
+  double beta1, beta2, eps, max_norm;
+  int32_t n_chunks, state_bits, grad_type, shadow_type;
+} mscl_adamw_desc;
+int mscl_adamw_step(const mscl_adamw_desc* d, void* stream);
+/* what 8-bit states stand for, as bf16 (exact) */
+int mscl_adamw_values(const uint8_t* m, const uint8_t* v, const uint8_t* exponents, uint16_t* m_out, uint16_t* v_out, int64_t n_blocks,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

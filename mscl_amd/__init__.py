@@ -7,6 +7,6 @@ __version__ = '0.1.0'
 
 from . import augment, heads, necks, recognizer3d, recognizers          # noqa: F401  (registration side effects)
 from .config import Config                                # noqa: F401
-from .optim import ClipSGD                                # noqa: F401
+from .optim import AdamW, ClipAdamW, ClipSGD, build_optimizer        # noqa: F401
 from .registry import (BACKBONES, HEADS, LOSSES, NECKS, RECOGNIZERS, SSL_AUGS, build_head, build_loss,   # noqa: F401
                        build_model, build_neck, build_recognizer, build_ssl_aug)

@@ -6,7 +6,7 @@ raises -- the product path never silently degrades to PyTorch ops.
 """
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_float, c_int, c_int64, c_void_p
+from ctypes import POINTER, Structure, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
 
@@ -26,6 +26,13 @@ class ConvDesc(Structure):
 class BnParams(Structure):
     _fields_ = [(n, c_void_p) for n in ('sum', 'sumsq', 'gamma', 'beta', 'running_mean', 'running_var',
                                         'num_batches_tracked', 'save_mean', 'save_invstd')]
+
+
+class AdamWDesc(Structure):
+    _fields_ = ([(n, c_void_p) for n in ('tensors', 'grads', 'chunk_tensor', 'm', 'v', 'exponents')] + [('n_blocks', c_int64)] +
+                [(n, c_void_p) for n in ('words', 'partials', 'grad_norm', 'lr')] +
+                [(n, c_double) for n in ('beta1', 'beta2', 'eps', 'max_norm')] +
+                [(n, c_int32) for n in ('n_chunks', 'state_bits', 'grad_type', 'shadow_type')])
 
 
 P = c_void_p
@@ -101,6 +108,8 @@ _SIGS = {
     'mscl_sumsq': [P, P, c_int64, P, c_int, P],
     'mscl_sgd_step': [P, P, P, P, c_int64, P, c_float, c_float, c_float, c_float, c_int, P],
     'mscl_cast_bf16': [P, P, c_int64, P],
+    'mscl_adamw_step': [POINTER(AdamWDesc), P],
+    'mscl_adamw_values': [P, P, P, P, P, c_int64, P],
 }
 _INT64_RESULT = ('mscl_debug_wgrad_stem_launches', 'mscl_debug_dgrad_s2_launches', 'mscl_debug_wgrad_group_launches', 'mscl_wgrad_halo_ws', 'mscl_debug_halo_launches', 'mscl_debug_stem_launches', 'mscl_debug_wgrad_halo_launches', 'mscl_det_parts_floats', 'mscl_conv3d_wgrad_ws', 'mscl_debug_pp_launches', 'mscl_debug_thin_launches', 'mscl_debug_k1_launches', 'mscl_debug_thin_wgrad_launches', 'mscl_wgrad_thin_ws')
 EXPORTS = tuple(_SIGS)

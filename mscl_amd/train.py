@@ -19,7 +19,7 @@ from collections import OrderedDict
 import torch
 
 from . import parallel
-from .optim import cosine_lr
+from .optim import ClipAdamW, cosine_lr
 
 
 def save_checkpoint(path, model, optimizer, epoch=0, it=0):
@@ -29,9 +29,12 @@ def save_checkpoint(path, model, optimizer, epoch=0, it=0):
                  'mscl_amd': {'rgb_iters': model.recognizer.iters, 'flow_iters': model.recognizer_flow.iters,
                               'step': model._step, 'optimizer_steps': optimizer.steps}},
         'state_dict': {k: v.detach().cpu().clone() for k, v in model.state_dict().items()},
-        'optimizer': {'momentum_buffer_flat': ar.MOM.detach().cpu().clone(), 'lr': optimizer.param_groups[0]['lr'],
-                      'momentum': optimizer.momentum, 'weight_decay': optimizer.wd},
     }
+    if isinstance(optimizer, ClipAdamW):
+        ckpt['optimizer'] = {k: v.cpu() if torch.is_tensor(v) else v for k, v in optimizer.state_dict().items()}
+    else:
+        ckpt['optimizer'] = {'momentum_buffer_flat': ar.MOM.detach().cpu().clone(), 'lr': optimizer.param_groups[0]['lr'],
+                             'momentum': optimizer.momentum, 'weight_decay': optimizer.wd}
     torch.save(ckpt, path)
     return ckpt['meta']
 
@@ -67,7 +70,12 @@ def resume(path, model, optimizer, restore_counters=True):
     model.load_state_dict(ckpt['state_dict'])
     model.sync_shadows()
     o = ckpt.get('optimizer') or {}
-    if 'momentum_buffer_flat' in o:
+    if isinstance(optimizer, ClipAdamW):
+        if 'slots' in o or any('exp_avg' in st for st in (o.get('state') or {}).values()):
+            optimizer.load_state_dict(o)
+        else:
+            warnings.warn('checkpoint holds no AdamW state: the moments restart at zero')
+    elif 'momentum_buffer_flat' in o:
         model.arena.MOM.copy_(o['momentum_buffer_flat'].to(model.arena.device))
         optimizer.param_groups[0]['lr'] = o['lr']
     elif 'state' in o:
