@@ -450,6 +450,40 @@ int mscl_adamw_step(const mscl_adamw_desc* d, void* stream);
 int mscl_adamw_values(const uint8_t* m, const uint8_t* v, const uint8_t* exponents, uint16_t* m_out, uint16_t* v_out, int64_t n_blocks,
                       void* stream);
 
+/* ---- residual norm (res_norm.hip) ---------------------------------------------------------------------------------------------
+ * What stands between two blocks of a residual network whose norms work on channels instead of batches, in one pass each way:
+ *   y = x + scale * act(gate) * (w_post * N_post(f) + b_post);   h = w_pre * N_pre(y) + b_pre
+ * N: RMS or layer norm over the C channels of a row (MSCL_NORM_*).  Rows are positions (N T H W of a map), x and f have row strides
+ * ld_x / ld_f in elements, everything else is dense.  Every part may be missing: f = NULL leaves h = N_pre(x) alone (no y); post / pre
+ * = 0 no norm; NULL scale, weights, biases, gate.  gate: (rows / rows_per_gate, C) of f's type, one row of gates for rows_per_gate
+ * consecutive rows (the positions of a clip; 1: a gate per element).  Types: x, y, dy, dx x_type; f, gate, h, dh, df, dgate f_type;
+ * (x_type, f_type) equal, or fp32 with a 16-bit f_type; per-channel vectors and statistics fp32.  C <= MSCL_RES_NORM_MAX_C, rows < 2^31.
+ * The forward writes the statistics that are not NULL; the backward wants those of the norms it goes through, x and f as in the forward,
+ * dy and / or dh, and writes the gradients that are not NULL -- per-channel ones added to what is there when accumulate != 0.
+ * Deterministic.  The BatchNorm counterpart is mscl_bn_act_fwd / _bwd. */
+#define MSCL_NORM_RMS   1
+#define MSCL_NORM_LAYER 2
+#define MSCL_GATE_LINEAR  0
+#define MSCL_GATE_SIGMOID 1
+#define MSCL_GATE_TANH    2
+#define MSCL_RES_NORM_MAX_C 16384
+typedef struct {
+  const void *x, *f, *gate;
+  const float *scale, *w_post, *b_post, *w_pre, *b_pre;
+  void *y, *h;
+  float *mean_f, *rstd_f, *mean_y, *rstd_y;          /* rows floats each */
+  const void *dy, *dh;
+  void *dx, *df, *dgate;
+  float *dscale, *dw_post, *db_post, *dw_pre, *db_pre;
+  float* ws; int64_t ws_floats;                      /* backward: mscl_res_norm_ws() floats */
+  int64_t rows, ld_x, ld_f, rows_per_gate;
+  int32_t C, x_type, f_type, post, pre, gate_act, accumulate;
+  float eps;
+} mscl_res_norm_desc;
+int mscl_res_norm_fwd(const mscl_res_norm_desc* d, void* stream);
+int64_t mscl_res_norm_ws(const mscl_res_norm_desc* d);
+int mscl_res_norm_bwd(const mscl_res_norm_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -571,3 +571,173 @@ def sgd_step(p, g, buf, p_bf16, sumsq_t, max_norm, lr, momentum, wd, first):
 
 def cast_bf16(src, dst):
     call('mscl_cast_bf16', ptr(src), ptr(dst), src.numel(), stream_ptr())
+
+
+# ---- residual norm (include/mscl_hip.h): y = x + scale * act(gate) * (w_post * N_post(f) + b_post), h = w_pre * N_pre(y) + b_pre
+NORMS = {None: 0, 'rms': 1, 'layer': 2}
+GATES = {'linear': 0, 'sigmoid': 1, 'tanh': 2}
+RES_NORM_MAX_C = 16384
+_TYPE_CODE = {torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+_VECTORS = ('scale', 'w_post', 'b_post', 'w_pre', 'b_pre')
+
+
+def _rows_of(t, C):
+    """(tensor, row stride) with t's rows C channels long, last dimension dense and all leading dimensions one stride apart; copies only
+    what no single row stride describes"""
+    if t.is_contiguous():
+        return t, C
+    if t.stride(-1) == 1 or C == 1:
+        at = None
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if at is None:
+                at = ld = stride
+            elif stride != at:
+                break
+            at *= size
+        else:
+            if at is None:
+                return t, C                              # one row
+            if ld >= C:
+                return t, ld
+    return t.contiguous(), C
+
+
+class ResNormSaved:
+    """what res_norm_bwd needs of a forward call"""
+    __slots__ = ('x', 'f', 'gate', 'vec', 'stats', 'codes', 'eps', 'shape', 'dims')
+
+
+def _res_norm_check(x, f, gate, vec, post_norm, pre_norm, gate_act, eps):
+    """refuses what the kernels do not take; returns (rows, C, rows per gate)"""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise lib.MsclError(f'res_norm: x has no channels: {tuple(x.shape)}')
+    C = x.shape[-1]
+    rows = x.numel() // C
+    if C > RES_NORM_MAX_C or rows >= 1 << 31:
+        raise lib.MsclError(f'res_norm takes up to {RES_NORM_MAX_C} channels and 2^31 - 1 rows, got {rows} x {C}')
+    if post_norm not in NORMS or pre_norm not in NORMS or gate_act not in GATES:
+        raise lib.MsclError(f'res_norm: norms are rms, layer or None, gates linear, sigmoid or tanh; got {post_norm}, {pre_norm}, {gate_act}')
+    if not eps > 0:
+        raise lib.MsclError('res_norm: eps > 0')
+    if f is None and (pre_norm is None or gate is not None or post_norm is not None or any(vec[k] is not None for k in ('scale', 'w_post', 'b_post'))):
+        raise lib.MsclError('res_norm: without a branch f only the norm before the next block (pre_norm, w_pre, b_pre) is left')
+    kind = x.dtype if f is None else f.dtype
+    if x.dtype not in _TYPE_CODE or kind not in _TYPE_CODE or (x.dtype != kind and x.dtype != torch.float32):
+        raise lib.MsclError(f'res_norm: fp32, bf16 or fp16, equal for x and f or x in fp32; got {x.dtype}, {kind}')
+    if f is not None and f.shape != x.shape:
+        raise lib.MsclError(f'res_norm: f {tuple(f.shape)} does not fit x {tuple(x.shape)}')
+    for k, v in vec.items():
+        if v is None:
+            continue
+        if v.dtype != torch.float32 or tuple(v.shape) != (C,) or not v.is_contiguous() or v.device != x.device:
+            raise lib.MsclError(f'res_norm: {k} is a contiguous fp32 vector of {C} channels beside x')
+        if (k.endswith('post') and post_norm is None) or (k.endswith('pre') and pre_norm is None):
+            raise lib.MsclError(f'res_norm: {k} without its norm')
+    per = 0
+    if gate is not None:
+        whole = gate.shape == x.shape
+        if gate.dtype != kind or gate.device != x.device or not (whole or (gate.dim() == 2 and gate.shape[1] == C)):
+            raise lib.MsclError(f"res_norm: gate is (gates, {C}) or like x, of f's type; got {tuple(gate.shape)} {gate.dtype}")
+        n = gate.numel() // C
+        if rows and (n == 0 or rows % n):
+            raise lib.MsclError(f'res_norm: {n} gates do not divide {rows} rows')
+        per = rows // n if n else 0
+    for t in (f, gate):
+        if t is not None and t.device != x.device:
+            raise lib.MsclError('res_norm: all tensors on one device')
+    return rows, C, per
+
+
+def res_norm_fwd(x, f=None, *, gate=None, gate_act='sigmoid', scale=None, post_norm=None, w_post=None, b_post=None, pre_norm=None, w_pre=None,
+                 b_pre=None, eps=1e-6, save=False):
+    """One pass over the rows of x (..., C): y = x + scale * act(gate) * (w_post * N_post(f) + b_post), h = w_pre * N_pre(y) + b_pre.
+    f None: h = norm of x alone (y is x).  Norms: 'rms', 'layer' or None; h is None without pre_norm.  gate: like x, or (gates, C) with
+    equal runs of consecutive rows per gate -- (N, C) for the clips of an NDHWC map.  x bf16 / fp16 / fp32; f and gate of x's type, or
+    16-bit beside an fp32 x; y has x's type, h f's.  Returns (y, h, saved); saved (save=True) is for res_norm_bwd."""
+    vec = dict(scale=scale, w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre)
+    rows, C, per = _res_norm_check(x, f, gate, vec, post_norm, pre_norm, gate_act, eps)
+    if not x.is_cuda:
+        raise lib.MsclError('mscl_amd kernels run on the GPU only (got a CPU tensor); there is no CPU fallback')
+    if torch.cuda.current_device() != x.device.index:
+        with torch.cuda.device(x.device):
+            return res_norm_fwd(x, f, gate=gate, gate_act=gate_act, post_norm=post_norm, pre_norm=pre_norm, eps=eps, save=save, **vec)
+    x, ld_x = _rows_of(x, C)
+    kind = x.dtype
+    y, ld_f = x, C
+    if f is not None:
+        kind = f.dtype
+        f, ld_f = _rows_of(f, C)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if gate is not None:
+        gate = gate.contiguous()
+    h = torch.empty(x.shape, dtype=kind, device=x.device) if pre_norm is not None else None
+    stats = [None] * 4                                   # mean_f, rstd_f, mean_y, rstd_y
+    if save:
+        want = (post_norm == 'layer', post_norm is not None, pre_norm == 'layer', pre_norm is not None)
+        stats = [torch.empty(rows, dtype=torch.float32, device=x.device) if w else None for w in want]
+    if rows:
+        d = lib.ResNormDesc(x=x.data_ptr(), f=ptr(f), gate=ptr(gate), scale=ptr(scale), w_post=ptr(w_post), b_post=ptr(b_post), w_pre=ptr(w_pre),
+                            b_pre=ptr(b_pre), y=ptr(y) if f is not None else None, h=ptr(h), mean_f=ptr(stats[0]), rstd_f=ptr(stats[1]),
+                            mean_y=ptr(stats[2]), rstd_y=ptr(stats[3]), rows=rows, ld_x=ld_x, ld_f=ld_f, rows_per_gate=per, C=C,
+                            x_type=_TYPE_CODE[x.dtype], f_type=_TYPE_CODE[kind], post=NORMS[post_norm], pre=NORMS[pre_norm],
+                            gate_act=GATES[gate_act], eps=eps)
+        call('mscl_res_norm_fwd', ctypes.byref(d), stream_ptr())
+    if not save:
+        return y, h, None
+    saved = ResNormSaved()
+    saved.x, saved.f, saved.gate, saved.vec, saved.stats, saved.eps, saved.shape = x, f, gate, vec, stats, eps, tuple(x.shape)
+    saved.codes, saved.dims = (NORMS[post_norm], NORMS[pre_norm], GATES[gate_act]), (rows, C, per, ld_x, ld_f)
+    return y, h, saved
+
+
+def res_norm_bwd(saved, dy=None, dh=None, into=None, need=None):
+    """Gradients of res_norm_fwd from dy (of y, or of x itself where there was no f) and / or dh.  Returns a dict with 'x', 'f', 'gate',
+    'scale', 'w_post', 'b_post', 'w_pre', 'b_pre' for what the forward was given (per-channel ones in fp32).  into: {name: fp32 vector} to
+    ADD those per-channel gradients to instead -- all of them or none.  need: names to compute (None: all)."""
+    x, f, gate, vec = saved.x, saved.f, saved.gate, saved.vec
+    rows, C, per, ld_x, ld_f = saved.dims
+    post, pre, act = saved.codes
+    kind = x.dtype if f is None else f.dtype
+    if dy is None and dh is None:
+        raise lib.MsclError('res_norm_bwd needs dy or dh')
+    if dh is not None and not pre:
+        raise lib.MsclError('res_norm_bwd: dh without pre_norm')
+    for g, t, what in ((dy, x.dtype, 'dy'), (dh, kind, 'dh')):
+        if g is not None and (tuple(g.shape) != saved.shape or g.dtype != t or g.device != x.device):
+            raise lib.MsclError(f'res_norm_bwd: {what} is {tuple(saved.shape)} {t}, got {tuple(g.shape)} {g.dtype}')
+    names = [k for k in ('x', 'f', 'gate') + _VECTORS if k == 'x' or (f if k == 'f' else gate if k == 'gate' else vec[k]) is not None]
+    names = [k for k in names if need is None or k in need]
+    if into is not None:
+        for k in names:
+            if k in _VECTORS and (k not in into or into[k].dtype != torch.float32 or into[k].numel() != C or not into[k].is_contiguous() or into[k].device != x.device):
+                raise lib.MsclError(f'res_norm_bwd: into[{k!r}] is a contiguous fp32 vector of {C} channels beside x')
+    if torch.cuda.current_device() != x.device.index:
+        with torch.cuda.device(x.device):
+            return res_norm_bwd(saved, dy, dh, into, need)
+    dy = dy.contiguous() if dy is not None else None
+    dh = dh.contiguous() if dh is not None else None
+    out = {}
+    for k in names:
+        if k in _VECTORS:
+            made = k.endswith('pre') and dh is None or rows == 0                 # nothing reaches it
+            out[k] = into[k] if into is not None else (torch.zeros if made else torch.empty)(C, dtype=torch.float32, device=x.device)
+        else:
+            src = x if k == 'x' else f if k == 'f' else gate
+            out[k] = torch.empty(src.shape, dtype=src.dtype, device=x.device)
+    if rows == 0:
+        return out
+    got = {k: ptr(v) for k, v in out.items()}
+    d = lib.ResNormDesc(x=x.data_ptr(), f=ptr(f), gate=ptr(gate), scale=ptr(vec['scale']), w_post=ptr(vec['w_post']), b_post=ptr(vec['b_post']),
+                        w_pre=ptr(vec['w_pre']), b_pre=ptr(vec['b_pre']), mean_f=ptr(saved.stats[0]), rstd_f=ptr(saved.stats[1]),
+                        mean_y=ptr(saved.stats[2]), rstd_y=ptr(saved.stats[3]), dy=ptr(dy), dh=ptr(dh), dx=got.get('x'), df=got.get('f'),
+                        dgate=got.get('gate'), dscale=got.get('scale'), dw_post=got.get('w_post'), db_post=got.get('b_post'),
+                        dw_pre=got.get('w_pre'), db_pre=got.get('b_pre'), rows=rows, ld_x=ld_x, ld_f=ld_f, rows_per_gate=per, C=C,
+                        x_type=_TYPE_CODE[x.dtype], f_type=_TYPE_CODE[kind], post=post, pre=pre, gate_act=act,
+                        accumulate=int(into is not None), eps=saved.eps)
+    n = lib.call_raw('mscl_res_norm_ws', ctypes.byref(d))
+    ws = torch.empty(n, dtype=torch.float32, device=x.device)
+    d.ws, d.ws_floats = ws.data_ptr(), n
+    call('mscl_res_norm_bwd', ctypes.byref(d), stream_ptr())
+    return out

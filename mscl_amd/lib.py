@@ -35,6 +35,13 @@ class AdamWDesc(Structure):
                 [(n, c_int32) for n in ('n_chunks', 'state_bits', 'grad_type', 'shadow_type')])
 
 
+class ResNormDesc(Structure):
+    _fields_ = ([(n, c_void_p) for n in ('x', 'f', 'gate', 'scale', 'w_post', 'b_post', 'w_pre', 'b_pre', 'y', 'h', 'mean_f', 'rstd_f', 'mean_y',
+                                         'rstd_y', 'dy', 'dh', 'dx', 'df', 'dgate', 'dscale', 'dw_post', 'db_post', 'dw_pre', 'db_pre', 'ws')] +
+                [(n, c_int64) for n in ('ws_floats', 'rows', 'ld_x', 'ld_f', 'rows_per_gate')] +
+                [(n, c_int32) for n in ('C', 'x_type', 'f_type', 'post', 'pre', 'gate_act', 'accumulate')] + [('eps', c_float)])
+
+
 P = c_void_p
 _SIGS = {
     'mscl_abi_version': [],
@@ -109,9 +116,12 @@ _SIGS = {
     'mscl_sgd_step': [P, P, P, P, c_int64, P, c_float, c_float, c_float, c_float, c_int, P],
     'mscl_cast_bf16': [P, P, c_int64, P],
     'mscl_adamw_step': [POINTER(AdamWDesc), P],
+    'mscl_res_norm_fwd': [POINTER(ResNormDesc), P],
+    'mscl_res_norm_ws': [POINTER(ResNormDesc)],
+    'mscl_res_norm_bwd': [POINTER(ResNormDesc), P],
     'mscl_adamw_values': [P, P, P, P, P, c_int64, P],
 }
-_INT64_RESULT = ('mscl_debug_wgrad_stem_launches', 'mscl_debug_dgrad_s2_launches', 'mscl_debug_wgrad_group_launches', 'mscl_wgrad_halo_ws', 'mscl_debug_halo_launches', 'mscl_debug_stem_launches', 'mscl_debug_wgrad_halo_launches', 'mscl_det_parts_floats', 'mscl_conv3d_wgrad_ws', 'mscl_debug_pp_launches', 'mscl_debug_thin_launches', 'mscl_debug_k1_launches', 'mscl_debug_thin_wgrad_launches', 'mscl_wgrad_thin_ws')
+_INT64_RESULT = ('mscl_res_norm_ws', 'mscl_debug_wgrad_stem_launches', 'mscl_debug_dgrad_s2_launches', 'mscl_debug_wgrad_group_launches', 'mscl_wgrad_halo_ws', 'mscl_debug_halo_launches', 'mscl_debug_stem_launches', 'mscl_debug_wgrad_halo_launches', 'mscl_det_parts_floats', 'mscl_conv3d_wgrad_ws', 'mscl_debug_pp_launches', 'mscl_debug_thin_launches', 'mscl_debug_k1_launches', 'mscl_debug_thin_wgrad_launches', 'mscl_wgrad_thin_ws')
 EXPORTS = tuple(_SIGS)
 
 _lib = None
