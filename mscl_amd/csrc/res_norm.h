@@ -1,0 +1,567 @@
+#pragma once
+// Residual norm: the channel norm that closes a block, the block's gate and residual scale, the residual add and the channel norm that
+// opens the next block, in one pass over the rows (gfx950, HBM-bound).  A row = the C channels of one position.
+//
+//   n = N_post(f)      rms: f r, r = 1 / sqrt(mean f^2 + eps);   layer: (f - mu) r, r = 1 / sqrt(mean (f - mu)^2 + eps);   none: f
+//   y = x + s a(gate) (w n + b)          h = N_pre(y) w' + b'        (h from y before y is rounded)
+// backward, from dy and dh, reads x, f and gate again and rebuilds y in fp32 -- the same bytes as reading y, and no rounding of y in the
+// weight gradients:
+//   t = dy + r' (dh w' - mean(dh w') - yhat mean(dh w' yhat))       dx = t
+//   d = t s a w;   df = r (d - mean(d) - n mean(d n))                (rms: no mean(d), mean(dh w') terms)
+//   dgate = s a' (w T1 + b T2) over the rows of a gate, T1 = sum t n, T2 = sum t;   with t1 = sum a T1, t2 = sum a T2 over the gates:
+//   ds = w t1 + b t2,  dw = s t1,  db = s t2;   dw' = sum dh yhat,  db' = sum dh
+// so two column sums carry the gradients of gate, scale, weight and bias.  No atomics: a block leaves one row of column sums per
+// accumulator, a second launch adds the rows in a fixed order in 64 bits.
+//
+// A TEAM of lanes owns a row: 1 .. 16 or 64 lanes of a wave (sums by DPP), or the whole block (sums through LDS).  A lane holds NV x 8
+// adjacent channels in registers, so a row is read once; the loads of a team's next row are in flight while it works on the current one.
+// Accesses are 16 bytes at the alignment of an element (the memory path of gfx950 takes any), so odd widths and strides run the same
+// code; only the lane with the last, partial 8 channels goes element by element.
+#include "common.h"
+#include <hip/hip_fp16.h>
+
+namespace {
+__device__ __forceinline__ float h2f(uint16_t h) { return __half2float(__ushort_as_half(h)); }
+__device__ __forceinline__ uint16_t f2h(float f) { return __half_as_ushort(__float2half_rn(f)); }
+template <int T> __device__ __forceinline__ float ld1(const void* p, int64_t e) {
+  if (T == MSCL_F32) return ((const float*)p)[e];
+  const uint16_t h = ((const uint16_t*)p)[e];
+  return T == MSCL_BF16 ? bf2f(h) : h2f(h);
+}
+template <int T> __device__ __forceinline__ void st1(void* p, int64_t e, float v) {
+  if (T == MSCL_F32) ((float*)p)[e] = v;
+  else ((uint16_t*)p)[e] = T == MSCL_BF16 ? f2bf(v) : f2h(v);
+}
+
+// 8 channels as they lie in memory
+template <int T> struct Raw { uint32_t w[T == MSCL_F32 ? 8 : 4]; };
+template <int T> __device__ __forceinline__ void unpack(const Raw<T>& u, float* v) {
+  if (T == MSCL_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u.w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = T == MSCL_BF16 ? __uint_as_float(u.w[i] << 16) : h2f((uint16_t)u.w[i]);
+      v[2 * i + 1] = T == MSCL_BF16 ? __uint_as_float(u.w[i] & 0xFFFF0000u) : h2f((uint16_t)(u.w[i] >> 16));
+    }
+  }
+}
+
+// a lane's channels of a row: value (q, i) is channel (q T + lane) 8 + i
+template <int NV> struct Cols {
+  int lane, T, C;
+  __device__ __forceinline__ int col(int q) const { return (q * T + lane) * 8; }
+  __device__ __forceinline__ int count(int q) const { const int n = C - col(q); return n < 0 ? 0 : n; }        // 8 or more: all
+  // channels past C read as zero
+  template <int TY> __device__ __forceinline__ void fetch(const void* p, int64_t row, Raw<TY> (&u)[NV]) const {
+    constexpr int sz = TY == MSCL_F32 ? 4 : 2;
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      const char* a = (const char*)p + (row + col(q)) * sz;
+      const int n = count(q);
+      if (n >= 8) {
+        if (TY == MSCL_F32) __builtin_memcpy(u[q].w, (const float*)a, 32);
+        else __builtin_memcpy(u[q].w, (const uint16_t*)a, 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < (TY == MSCL_F32 ? 8 : 4); ++i) u[q].w[i] = 0;
+        if (n > 0) {
+#pragma unroll
+          for (int i = 0; i < 7; ++i)
+            if (i < n) {
+              if (TY == MSCL_F32) u[q].w[i] = ((const uint32_t*)a)[i];
+              else u[q].w[i >> 1] |= (uint32_t)((const uint16_t*)a)[i] << (16 * (i & 1));
+            }
+        }
+      }
+    }
+  }
+  template <int TY> __device__ __forceinline__ void load(const void* p, int64_t row, float (&v)[NV][8]) const {
+    Raw<TY> u[NV];
+    fetch<TY>(p, row, u);
+#pragma unroll
+    for (int q = 0; q < NV; ++q) unpack<TY>(u[q], v[q]);
+  }
+  // a per-channel vector; a missing one is all `one`.  Zero past C, so that those channels add nothing to a row's sums
+  __device__ __forceinline__ void load_vec(const float* p, float one, float (&v)[NV][8]) const {
+    if (p) load<MSCL_F32>(p, 0, v);
+    else
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[q][i] = i < count(q) ? one : 0.f;
+  }
+  template <int TY> __device__ __forceinline__ void store(void* p, int64_t row, const float (&v)[NV][8]) const {
+    constexpr int sz = TY == MSCL_F32 ? 4 : 2;
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      char* a = (char*)p + (row + col(q)) * sz;
+      const int n = count(q);
+      if (n >= 8) {
+        if (TY == MSCL_F32) __builtin_memcpy((float*)a, v[q], 32);
+        else {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = TY == MSCL_BF16 ? pack2bf(v[q][2 * i], v[q][2 * i + 1]) : (uint32_t)f2h(v[q][2 * i]) | (uint32_t)f2h(v[q][2 * i + 1]) << 16;
+          __builtin_memcpy((uint16_t*)a, w, 16);
+        }
+      } else if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < 7; ++i) if (i < n) st1<TY>(a, i, v[q][i]);
+      }
+    }
+  }
+};
+
+// team sums.  WAVE: T in {1, 2, 4, 8, 16, 64}.  Block teams: waves meet in LDS; two alternating slots make one barrier per sum enough
+// (a slot is written again only by waves that have passed the barrier of the sum between, i.e. after every wave has read it).
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+template <bool WAVE> struct Team {
+  int T;
+  float2* red;          // block teams: [2][16]
+  int slot;
+  __device__ __forceinline__ float wsum(float v) const {
+    if (T == 64) return wave_sum(v);
+    if (T >= 2) v = dpp_add<0xB1>(v);        // quad_perm: neighbour
+    if (T >= 4) v = dpp_add<0x4E>(v);        // quad_perm: other pair
+    if (T >= 8) v = dpp_add<0x141>(v);       // row_half_mirror: other quad
+    if (T >= 16) v = dpp_add<0x128>(v);      // row_ror 8: other half row
+    return v;
+  }
+  __device__ __forceinline__ float2 sum2(float a, float b, bool want_b) {
+    if (WAVE) return make_float2(wsum(a), want_b ? wsum(b) : 0.f);
+    a = wave_sum(a);
+    if (want_b) b = wave_sum(b);
+    const int w = threadIdx.x >> 6, nw = blockDim.x >> 6, l = threadIdx.x & 15;
+    float2* s = red + slot * 16;
+    slot ^= 1;
+    if ((threadIdx.x & 63) == 0) s[w] = make_float2(a, b);
+    __syncthreads();
+    const float2 t = l < nw ? s[l] : make_float2(0.f, 0.f);          // every 16 lanes add the (at most 16) waves' values
+    return make_float2(row16_sum(t.x), want_b ? row16_sum(t.y) : 0.f);
+  }
+  __device__ __forceinline__ float sum(float a) { return sum2(a, 0.f, false).x; }
+};
+
+__device__ __forceinline__ float act_fwd(int act, float g) {
+  if (act == MSCL_GATE_SIGMOID) return 1.f / (1.f + expf(-g));
+  if (act == MSCL_GATE_TANH) return tanhf(g);
+  return g;
+}
+// a'(g) = e / (1 + e)^2 with e = exp(-|g|) (sigmoid), 4 e / (1 + e)^2 with e = exp(-2 |g|) (tanh): no difference of near numbers, which
+// a (1 - a) and 1 - a^2 are for a saturated gate
+__device__ __forceinline__ float act_slope(int act, float g) {
+  if (act == MSCL_GATE_LINEAR) return 1.f;
+  const bool th = act == MSCL_GATE_TANH;
+  const float e = expf(-fabsf(g) * (th ? 2.f : 1.f)), q = 1.f / (1.f + e);
+  return (th ? 4.f : 1.f) * e * q * q;
+}
+
+#define EACH _Pragma("unroll") for (int q = 0; q < NV; ++q) _Pragma("unroll") for (int i = 0; i < 8; ++i)
+
+// mean and 1 / deviation of a row held in v (rms: mean 0); the second moment is taken about the mean, in a second pass over registers
+template <int NV, bool WAVE>
+__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], int kind, float inv_c, float eps, const Cols<NV>& c, Team<WAVE>& team) {
+  float mu = 0.f, s = 0.f;
+  if (kind == MSCL_NORM_LAYER) {
+    EACH s += v[q][i];              // channels past C are zero
+    mu = team.sum(s) * inv_c;
+    s = 0.f;
+    EACH { const float d = i < c.count(q) ? v[q][i] - mu : 0.f; s += d * d; }
+  } else {
+    EACH s += v[q][i] * v[q][i];
+  }
+  return make_float2(mu, 1.f / sqrtf(team.sum(s) * inv_c + eps));
+}
+}  // namespace
+
+// A block takes `share` consecutive rows, its teams in turn.  EACH_GATE: a gate for every row, fetched with it; otherwise the gate's
+// activation stays in registers until a row belongs to another gate.  BIAS: b_post or b_pre present.
+template <int XT, int FT, int NV, bool WAVE, bool EACH_GATE, bool BIAS>
+__global__ __launch_bounds__(WAVE ? 256 : 1024) void res_norm_fwd_kernel(mscl_res_norm_desc d, int T, FastDiv gdiv, int64_t share) {
+  __shared__ float2 red[32];
+  Team<WAVE> team{T, red, 0};
+  const int per = WAVE ? 256 / T : 1, sub = WAVE ? (int)threadIdx.x / T : 0;
+  const Cols<NV> c{WAVE ? (int)threadIdx.x % T : (int)threadIdx.x, T, d.C};
+  const float inv_c = 1.f / (float)d.C;
+  const int64_t end = share * (blockIdx.x + 1) < d.rows ? share * (blockIdx.x + 1) : d.rows;
+  int64_t r = share * blockIdx.x + sub;
+  Raw<XT> ux[NV];
+  Raw<FT> uf[NV], ug[NV];
+  if (r < end) {
+    c.template fetch<XT>(d.x, r * d.ld_x, ux);
+    if (d.f) c.template fetch<FT>(d.f, r * d.ld_f, uf);
+    if (EACH_GATE) c.template fetch<FT>(d.gate, r * d.C, ug);
+  }
+  float sw[NV][8], sb[BIAS ? NV : 1][8], w2[NV][8], b2[BIAS ? NV : 1][8], a[NV][8];
+  if (d.f) {
+    c.load_vec(d.scale, 1.f, a);
+    c.load_vec(d.w_post, 1.f, sw);
+    EACH sw[q][i] *= a[q][i];
+    if constexpr (BIAS) {
+      c.load_vec(d.b_post, 0.f, sb);
+      EACH sb[q][i] *= a[q][i];
+    }
+    EACH a[q][i] = 1.f;
+  }
+  if (d.pre) {
+    c.load_vec(d.w_pre, 1.f, w2);
+    if constexpr (BIAS) c.load_vec(d.b_pre, 0.f, b2);
+  }
+  int gate = -1;
+  for (; r < end; r += per) {
+    float x[NV][8], f[NV][8];
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      unpack<XT>(ux[q], x[q]);
+      if (d.f) unpack<FT>(uf[q], f[q]);
+      if (EACH_GATE) unpack<FT>(ug[q], a[q]);
+    }
+    if (r + per < end) {
+      c.template fetch<XT>(d.x, (r + per) * d.ld_x, ux);
+      if (d.f) c.template fetch<FT>(d.f, (r + per) * d.ld_f, uf);
+      if (EACH_GATE) c.template fetch<FT>(d.gate, (r + per) * d.C, ug);
+    }
+    if (d.f) {
+      if (EACH_GATE) {
+        EACH a[q][i] = act_fwd(d.gate_act, a[q][i]);
+      } else if (d.gate) {
+        const int g = fdiv((int)r, gdiv);
+        if (g != gate) {
+          gate = g;
+          c.template load<FT>(d.gate, (int64_t)g * d.C, a);
+          EACH a[q][i] = act_fwd(d.gate_act, a[q][i]);
+        }
+      }
+      if (d.post) {
+        const float2 st = row_stats<NV, WAVE>(f, d.post, inv_c, d.eps, c, team);
+        if (c.lane == 0) {
+          if (d.mean_f) d.mean_f[r] = st.x;
+          if (d.rstd_f) d.rstd_f[r] = st.y;
+        }
+        EACH f[q][i] = (f[q][i] - st.x) * st.y;
+      }
+      EACH x[q][i] += a[q][i] * (BIAS ? sw[q][i] * f[q][i] + sb[BIAS ? q : 0][i] : sw[q][i] * f[q][i]);       // zero past C: sw, sb are
+      c.template store<XT>(d.y, r * d.C, x);
+    }
+    if (d.pre) {
+      const float2 st = row_stats<NV, WAVE>(x, d.pre, inv_c, d.eps, c, team);
+      if (c.lane == 0) {
+        if (d.mean_y) d.mean_y[r] = st.x;
+        if (d.rstd_y) d.rstd_y[r] = st.y;
+      }
+      EACH { x[q][i] = (x[q][i] - st.x) * st.y * w2[q][i]; if (BIAS) x[q][i] += b2[BIAS ? q : 0][i]; }
+      c.template store<FT>(d.h, r * d.C, x);
+    }
+  }
+}
+
+// Which rows a block of the backward pass takes, and which column sums it leaves.
+//   SPLIT  the gates are long runs of rows (or there is one, or none): `per_gate` blocks share the rows of a gate, their T1 / T2 stay
+//          apart per gate until the second launch has added them up and applied a and a'
+//   WHOLE  the gates are short or very many: a team takes whole gates, applies a itself and writes dgate at the end of each
+//   EACH1  a gate for every row: as WHOLE with runs of one row, and nothing to keep between rows but the totals
+enum { SPLIT = 0, WHOLE = 1, EACH1 = 2 };
+struct BwdPlan { int T, wave, nv, mode, per_gate, gates, blocks, rows_per_gate; };
+
+template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS>
+__global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_desc d, BwdPlan pl) {
+  extern __shared__ float lds[];                    // wave teams: [256][8 NV] for the column sums of a block
+  __shared__ float2 red[32];
+  constexpr int NB = BIAS ? NV : 1;
+  const int T = pl.T;
+  Team<WAVE> team{T, red, 0};
+  const int per = WAVE ? 256 / T : 1, sub = WAVE ? (int)threadIdx.x / T : 0;
+  const Cols<NV> c{WAVE ? (int)threadIdx.x % T : (int)threadIdx.x, T, d.C};
+  const float inv_c = 1.f / (float)d.C;
+  const bool layer2 = d.pre == MSCL_NORM_LAYER, layer1 = d.post == MSCL_NORM_LAYER;
+
+  // the team's rows: r, r + step, ... < end; WHOLE: runs of rows_per_gate rows
+  int64_t r, step, end, gate = 0;
+  if (MODE == SPLIT) {
+    const int64_t g = blockIdx.x / pl.per_gate, j = blockIdx.x % pl.per_gate;
+    const int64_t share = (pl.rows_per_gate + pl.per_gate - 1) / pl.per_gate, r0 = g * pl.rows_per_gate;
+    end = r0 + (share * (j + 1) < pl.rows_per_gate ? share * (j + 1) : pl.rows_per_gate);
+    r = r0 + share * j + sub;
+    step = per;
+    gate = g;
+  } else {
+    gate = (int64_t)blockIdx.x * per + sub;
+    step = (int64_t)gridDim.x * per;                // in gates
+    r = gate * pl.rows_per_gate;
+    end = d.rows;
+  }
+  auto after = [&](int64_t at) {
+    if (MODE != WHOLE) return at + step;
+    return (at + 1) % pl.rows_per_gate ? at + 1 : at + 1 + (step - 1) * pl.rows_per_gate;
+  };
+  Raw<XT> ux[NV], uy[NV];
+  Raw<FT> uf[NV], uh[NV], ug[NV];
+  float sd[4] = {0.f, 1.f, 0.f, 1.f};               // mean_f, rstd_f, mean_y, rstd_y of the row that is on its way
+  auto fetch = [&](int64_t at) {
+    c.template fetch<XT>(d.x, at * d.ld_x, ux);
+    if (d.f) c.template fetch<FT>(d.f, at * d.ld_f, uf);
+    if (d.dy) c.template fetch<XT>(d.dy, at * d.C, uy);
+    if (d.dh) c.template fetch<FT>(d.dh, at * d.C, uh);
+    if (MODE == EACH1) c.template fetch<FT>(d.gate, at * d.C, ug);
+    if (d.f && d.post) { if (layer1) sd[0] = d.mean_f[at]; sd[1] = d.rstd_f[at]; }
+    if (d.dh) { if (layer2) sd[2] = d.mean_y[at]; sd[3] = d.rstd_y[at]; }
+  };
+  if (r < end) fetch(r);
+
+  float sw[NV][8], sb[NB][8], w2[NV][8], a[NV][8];
+  float U1[NV][8] = {}, U2[NB][8] = {}, T1[NV][8] = {}, T2[NB][8] = {}, t1[MODE == WHOLE ? NV : 1][8] = {}, t2[MODE == WHOLE ? NB : 1][8] = {};
+  if (d.f) {
+    c.load_vec(d.scale, 1.f, a);
+    c.load_vec(d.w_post, 1.f, sw);
+    EACH sw[q][i] *= a[q][i];
+    if constexpr (BIAS) {
+      c.load_vec(d.b_post, 0.f, sb);
+      EACH sb[q][i] *= a[q][i];
+    }
+    EACH a[q][i] = 1.f;
+  }
+  if (d.dh) c.load_vec(d.w_pre, 1.f, w2);
+  if (MODE == SPLIT && d.gate) {
+    c.template load<FT>(d.gate, gate * d.C, a);
+    EACH a[q][i] = act_fwd(d.gate_act, a[q][i]);
+  }
+  int64_t loaded = -1;
+
+  while (r < end) {
+    float x[NV][8], n[NV][8], t[NV][8], g[NV][8];
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      unpack<XT>(ux[q], x[q]);
+      if (d.f) unpack<FT>(uf[q], n[q]);
+      if (d.dy) unpack<XT>(uy[q], t[q]);
+      if (d.dh) unpack<FT>(uh[q], g[q]);
+      if (MODE == EACH1) unpack<FT>(ug[q], a[q]);
+    }
+    const float mu1 = sd[0], r1 = sd[1], mu2 = sd[2], r2 = sd[3];
+    const int64_t next = after(r);
+    if (next < end) fetch(next);
+    if (!d.dy) EACH t[q][i] = 0.f;
+    float logit[MODE == EACH1 ? NV : 1][8];
+    if constexpr (MODE == EACH1) {
+      EACH { logit[q][i] = a[q][i]; a[q][i] = act_fwd(d.gate_act, a[q][i]); }
+    }
+    if constexpr (MODE == WHOLE) {
+      if (gate != loaded) {
+        loaded = gate;
+        c.template load<FT>(d.gate, gate * d.C, a);
+        EACH a[q][i] = act_fwd(d.gate_act, a[q][i]);
+      }
+    }
+    if (d.f) {
+      if (d.post) EACH n[q][i] = (n[q][i] - mu1) * r1;
+      if (d.dh) EACH x[q][i] += a[q][i] * (BIAS ? sw[q][i] * n[q][i] + sb[BIAS ? q : 0][i] : sw[q][i] * n[q][i]);        // y
+    }
+    if (d.dh) {
+      float c1 = 0.f, c0 = 0.f;
+      EACH {
+        const float yh = (x[q][i] - mu2) * r2;      // past C: dh and w2 are zero, nothing of yh reaches a sum
+        x[q][i] = yh;
+        U1[q][i] += g[q][i] * yh;
+        if (BIAS) U2[BIAS ? q : 0][i] += g[q][i];
+        g[q][i] *= w2[q][i];
+        c1 += g[q][i] * yh;
+        if (layer2) c0 += g[q][i];
+      }
+      const float2 s = team.sum2(c1, c0, layer2);
+      const float m1 = s.x * inv_c, m0 = s.y * inv_c;
+      EACH t[q][i] += r2 * (g[q][i] - m0 - x[q][i] * m1);
+    }
+    if (d.dx) c.template store<XT>(d.dx, r * d.C, t);
+    if (d.f) {
+      float k1 = 0.f, k0 = 0.f;
+      EACH {
+        const float ti = t[q][i], tn = ti * n[q][i];
+        if (MODE == EACH1) {
+          T1[q][i] += a[q][i] * tn;
+          if (BIAS) T2[BIAS ? q : 0][i] += a[q][i] * ti;
+          logit[MODE == EACH1 ? q : 0][i] = act_slope(d.gate_act, logit[MODE == EACH1 ? q : 0][i]) * (BIAS ? sw[q][i] * tn + sb[BIAS ? q : 0][i] * ti : sw[q][i] * tn);
+        } else {
+          T1[q][i] += tn;
+          if (BIAS) T2[BIAS ? q : 0][i] += ti;
+        }
+        t[q][i] = ti * a[q][i] * sw[q][i];          // zero past C: sw is
+        k1 += t[q][i] * n[q][i];
+        if (layer1) k0 += t[q][i];
+      }
+      if constexpr (MODE == EACH1) { if (d.dgate) c.template store<FT>(d.dgate, r * d.C, logit); }
+      if (d.df) {
+        if (d.post) {
+          const float2 s = team.sum2(k1, k0, layer1);
+          const float m1 = s.x * inv_c, m0 = s.y * inv_c;
+          EACH t[q][i] = r1 * (t[q][i] - m0 - n[q][i] * m1);
+        }
+        c.template store<FT>(d.df, r * d.C, t);
+      }
+      if constexpr (MODE == WHOLE) {
+        if (next != r + 1 || next >= end || pl.rows_per_gate == 1) {        // the gate's last row
+          c.template load<FT>(d.gate, gate * d.C, x);
+          EACH {
+            const float s1 = T1[q][i], s2 = BIAS ? T2[BIAS ? q : 0][i] : 0.f;
+            t1[q][i] += a[q][i] * s1;
+            T1[q][i] = 0.f;
+            if (BIAS) { t2[BIAS ? q : 0][i] += a[q][i] * s2; T2[BIAS ? q : 0][i] = 0.f; }
+            x[q][i] = act_slope(d.gate_act, x[q][i]) * (BIAS ? sw[q][i] * s1 + sb[BIAS ? q : 0][i] * s2 : sw[q][i] * s1);
+          }
+          if (d.dgate) c.template store<FT>(d.dgate, gate * d.C, x);
+          gate += step;
+        }
+      }
+    }
+    r = next;
+  }
+
+  // the block's column sums: [4][C] floats (U1, U2, T1, T2; with the gates applied: t1, t2 in the place of T1, T2)
+  float* out = d.ws + (int64_t)blockIdx.x * 4 * d.C;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (!BIAS && (k & 1)) continue;
+    if (k < 2 ? !d.dh : !d.f) continue;             // block-uniform
+    float v[NV][8];
+    EACH v[q][i] = k == 0 ? U1[q][i] : k == 1 ? U2[BIAS ? q : 0][i] : k == 2 ? (MODE == WHOLE ? t1[MODE == WHOLE ? q : 0][i] : T1[q][i])
+                 : (MODE == WHOLE ? t2[MODE == WHOLE && BIAS ? q : 0][i] : T2[BIAS ? q : 0][i]);
+    if (!WAVE) { c.template store<MSCL_F32>(out + (int64_t)k * d.C, 0, v); continue; }
+    __syncthreads();
+    EACH lds[sub * T * 8 * NV + c.col(q) + i] = v[q][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < d.C; e += 256) {
+      float s = 0.f;
+      for (int u = 0; u < per; ++u) s += lds[u * T * 8 * NV + e];
+      out[(int64_t)k * d.C + e] = s;
+    }
+  }
+}
+#undef EACH
+
+// Adds the blocks' column sums: 16 columns x 64 lanes per block, in 64 bits and in a fixed order.  Split gates: lanes_per_gate lanes share
+// the blocks of a gate, the first of them writes dgate and goes on with a T1, a T2.
+template <int FT>
+__global__ __launch_bounds__(1024) void res_norm_finish_kernel(mscl_res_norm_desc d, BwdPlan pl, int lanes_per_gate) {
+  __shared__ double red[4][64][16];
+  const int cl = threadIdx.x & 15, lane = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + cl;
+  const bool in = col < d.C, split = pl.mode == SPLIT && d.gate;
+  const int64_t stride = (int64_t)4 * d.C;
+  const bool want[4] = {d.dh && d.dw_pre, d.dh && d.db_pre, d.f && !split, d.f && !split && d.b_post};
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+  if (in)
+#pragma unroll 4
+    for (int b = lane; b < pl.blocks; b += 64) {
+      const float* p = d.ws + b * stride + col;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) if (want[k]) v[k] += (double)p[(int64_t)k * d.C];
+    }
+  const double w = in && d.w_post ? (double)d.w_post[col] : 1.0, b = in && d.b_post ? (double)d.b_post[col] : 0.0;
+  const double s = in && d.scale ? (double)d.scale[col] : 1.0;
+  if (split) {
+    const int at_once = 64 / lanes_per_gate, mine = lane / lanes_per_gate, part = lane % lanes_per_gate;
+    for (int g0 = 0; g0 < pl.gates; g0 += at_once) {
+      const int g = g0 + mine;
+      double s1 = 0.0, s2 = 0.0;
+      if (in && g < pl.gates)
+#pragma unroll 4
+        for (int j = part; j < pl.per_gate; j += lanes_per_gate) {
+          const float* p = d.ws + ((int64_t)g * pl.per_gate + j) * stride + col;
+          s1 += (double)p[2 * (int64_t)d.C];
+          if (d.b_post) s2 += (double)p[3 * (int64_t)d.C];
+        }
+      if (lanes_per_gate > 1) {
+        __syncthreads();
+        red[0][lane][cl] = s1;
+        red[1][lane][cl] = s2;
+        __syncthreads();
+        if (part == 0)
+          for (int i = 1; i < lanes_per_gate; ++i) { s1 += red[0][lane + i][cl]; s2 += red[1][lane + i][cl]; }
+      }
+      if (part == 0 && in && g < pl.gates) {
+        const float logit = ld1<FT>(d.gate, (int64_t)g * d.C + col), a = act_fwd(d.gate_act, logit);
+        v[2] += (double)a * s1;
+        v[3] += (double)a * s2;
+        if (d.dgate) st1<FT>(d.dgate, (int64_t)g * d.C + col, (float)(s * (double)act_slope(d.gate_act, logit) * (w * s1 + b * s2)));
+      }
+    }
+    __syncthreads();
+  }
+  // over the 64 lanes of a column: 4 inside a wave, then 16 waves through LDS
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[k] += __shfl_xor(v[k], 16, 64);
+    v[k] += __shfl_xor(v[k], 32, 64);
+    if ((lane & 3) == 0) red[k][lane >> 2][cl] = v[k];
+  }
+  __syncthreads();
+  if (threadIdx.x >= 16 || !in) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[k] = 0.0;
+    for (int i = 0; i < 16; ++i) v[k] += red[k][i][cl];
+  }
+  auto put = [&](float* p, double x) { if (p) p[col] = (float)((d.accumulate ? (double)p[col] : 0.0) + x); };
+  if (d.dh) { put(d.dw_pre, v[0]); put(d.db_pre, v[1]); }
+  if (d.f) { put(d.dscale, w * v[2] + b * v[3]); put(d.dw_post, s * v[2]); put(d.db_post, s * v[3]); }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- launches
+// lanes, kind of team and channels per lane for rows of C channels (res_norm.hip)
+void res_norm_team(int C, int max_wave_nv, int* T, int* wave, int* nv);
+template <int XT, int FT, int NV, bool WAVE>
+static void fwd_launch(const mscl_res_norm_desc& d, int T, unsigned grid, int64_t share, hipStream_t st) {
+  const bool each = d.gate && d.rows_per_gate == 1, bias = d.b_post || d.b_pre;
+  const FastDiv g = make_fastdiv(d.gate ? (int)d.rows_per_gate : 1);
+  const dim3 th(WAVE ? 256 : T);
+  if (each) { if (bias) hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, true, true>), dim3(grid), th, 0, st, d, T, g, share);
+              else hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, true, false>), dim3(grid), th, 0, st, d, T, g, share); }
+  else { if (bias) hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, false, true>), dim3(grid), th, 0, st, d, T, g, share);
+         else hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, false, false>), dim3(grid), th, 0, st, d, T, g, share); }
+}
+template <int XT, int FT>
+void res_norm_fwd_types(const mscl_res_norm_desc& d, hipStream_t st) {
+  int T, wave, nv;
+  res_norm_team(d.C, 2, &T, &wave, &nv);
+  const int per = wave ? 256 / T : 1;
+  // blocks for 256 CUs of 32 waves; each takes its rows in one stretch
+  int64_t grid = wave ? 2048 : 8192 / (T / 64);
+  if (grid > cdiv64(d.rows, per)) grid = cdiv64(d.rows, per);
+  const int64_t share = cdiv64(cdiv64(d.rows, grid), per) * per;
+  grid = cdiv64(d.rows, share);
+  if (wave) { if (nv == 1) fwd_launch<XT, FT, 1, true>(d, T, (unsigned)grid, share, st); else fwd_launch<XT, FT, 2, true>(d, T, (unsigned)grid, share, st); }
+  else { if (nv == 1) fwd_launch<XT, FT, 1, false>(d, T, (unsigned)grid, share, st); else fwd_launch<XT, FT, 2, false>(d, T, (unsigned)grid, share, st); }
+}
+template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS>
+static void bwd_go(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
+  hipLaunchKernelGGL((res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS>), dim3(p.blocks), dim3(WAVE ? 256 : p.T), WAVE ? 256 * 8 * NV * 4 : 0, st, d, p);
+}
+template <int XT, int FT, int NV, bool WAVE, int THREADS>
+static void bwd_launch(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
+  // the rare forms (rows past 8192 channels, short runs per gate) carry the bias sums always
+  if (p.mode == WHOLE) return bwd_go<XT, FT, NV, WAVE, THREADS, WHOLE, true>(d, p, st);
+  if (NV > 1 || d.b_post || d.b_pre) {
+    if (p.mode == SPLIT) bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, true>(d, p, st);
+    else bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, true>(d, p, st);
+  } else if constexpr (NV == 1) {
+    if (p.mode == SPLIT) bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, false>(d, p, st);
+    else bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, false>(d, p, st);
+  }
+}
+template <int XT, int FT>
+int res_norm_bwd_types(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
+  if (p.wave) bwd_launch<XT, FT, 1, true, 256>(d, p, st);
+  else if (p.nv == 2) bwd_launch<XT, FT, 2, false, 1024>(d, p, st);
+  else if (p.T <= 512) bwd_launch<XT, FT, 1, false, 512>(d, p, st);
+  else bwd_launch<XT, FT, 1, false, 1024>(d, p, st);
+  MSCL_LAUNCH_CHECK();
+  int lanes = 1;
+  if (d.gate && p.mode == SPLIT) while (lanes * 2 * p.gates <= 64 && lanes * 2 <= p.per_gate) lanes *= 2;
+  hipLaunchKernelGGL(res_norm_finish_kernel<FT>, dim3((d.C + 15) / 16), dim3(1024), 0, st, d, p, lanes);
+  MSCL_LAUNCH_CHECK();
+  return 0;
+}
