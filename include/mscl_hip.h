@@ -408,7 +408,7 @@ int mscl_cast_bf16(const float* src, uint16_t* dst, int64_t n, void* stream);
 /* ---- AdamW over many tensors, moments in 32 or in 8 bits (adamw.hip) --------------------------------------------------------
  * torch.optim.AdamW (decoupled decay, amsgrad off), which mmcv's build_optimizer wires for `optimizer=dict(type='AdamW', ...)`
  * (mmaction/apis/train.py:94), with clip_grad_norm_ over all tensors ahead of it (mmcv OptimizerHook, apis/train.py:111-119) and the
- * per-parameter multipliers of `paramwise_cfg`.  Two launches whatever the number of tensors.
+ * per-parameter multipliers of `paramwise_cfg`.  Two or three launches whatever the number of tensors.
  *   step t = ++words.step;  c = min(1, max_norm / (|g| + 1e-6)) (1 when max_norm <= 0), *grad_norm = |g| before the clip;
  *   m = b1 m + (1-b1) c g;  v = b2 v + (1-b2) (c g)^2;
  *   p = p (1 - lr lr_mult decay) - lr lr_mult / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps);  shadow = round(p)
@@ -424,8 +424,8 @@ int mscl_cast_bf16(const float* src, uint16_t* dst, int64_t n, void* stream);
 #define MSCL_F16  3
 #define MSCL_ADAMW_BLOCK 256       /* elements that share an exponent; alignment of a tensor inside the state buffers */
 #define MSCL_ADAMW_CHUNK 4096      /* elements per entry of chunk_tensor (the last chunk of a tensor may be short) */
-#define MSCL_ADAMW_PARTS 256       /* doubles in `partials` */
-#define MSCL_ADAMW_WORDS 32        /* bytes in `words`: int64 step, 8 bytes derived from it, uint32 derived, uint32 seed at byte 20 */
+#define MSCL_ADAMW_PARTS 2048      /* doubles in `partials` */
+#define MSCL_ADAMW_WORDS 32        /* bytes in `words`, zeroed by the caller but for: int64 step at byte 0, uint32 seed at byte 20 */
 typedef struct {
   float* p;                 /* fp32 parameter, n elements */
   uint16_t* shadow;         /* 16-bit copy to refresh, or NULL when shadow_type is MSCL_NONE */

@@ -147,19 +147,27 @@ template <bool WAVE> struct Team {
   __device__ __forceinline__ float sum(float a) { return sum2(a, 0.f, false).x; }
 };
 
-__device__ __forceinline__ float act_fwd(int act, float g) {
-  if (act == MSCL_GATE_SIGMOID) return 1.f / (1.f + expf(-g));
-  if (act == MSCL_GATE_TANH) return tanhf(g);
-  return g;
+// exp(x) for x <= 0 to about 2 ulp: the rounding of x log2(e) is put back to first order
+__device__ __forceinline__ float exp_neg(float x) {
+  const float t = x * 1.44269504f, lo = fmaf(x, 1.92596303e-8f, fmaf(x, 1.44269504f, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, lo * 0.693147181f, e);
 }
-// a'(g) = e / (1 + e)^2 with e = exp(-|g|) (sigmoid), 4 e / (1 + e)^2 with e = exp(-2 |g|) (tanh): no difference of near numbers, which
-// a (1 - a) and 1 - a^2 are for a saturated gate
-__device__ __forceinline__ float act_slope(int act, float g) {
-  if (act == MSCL_GATE_LINEAR) return 1.f;
-  const bool th = act == MSCL_GATE_TANH;
-  const float e = expf(-fabsf(g) * (th ? 2.f : 1.f)), q = 1.f / (1.f + e);
-  return (th ? 4.f : 1.f) * e * q * q;
+// gate value a(g) and slope a'(g).  With e = exp(-|g|), q = 1 / (1 + e): sigmoid is q or e q by the sign of g, its slope e q^2; tanh's slope
+// 4 e q^2 with e = exp(-2 |g|).  No difference of near numbers, which a (1 - a) and 1 - a^2 are for a saturated gate.  (q: the 1-ulp reciprocal.)
+__device__ __forceinline__ float2 act_both(int act, float g) {
+  if (act == MSCL_GATE_SIGMOID) {
+    const float e = exp_neg(-fabsf(g)), q = __builtin_amdgcn_rcpf(1.f + e), eq = e * q;
+    return make_float2(g >= 0.f ? q : eq, eq * q);
+  }
+  if (act == MSCL_GATE_TANH) {
+    const float e = exp_neg(-2.f * fabsf(g)), q = __builtin_amdgcn_rcpf(1.f + e);
+    return make_float2(tanhf(g), 4.f * e * q * q);
+  }
+  return make_float2(g, 1.f);
 }
+__device__ __forceinline__ float act_fwd(int act, float g) { return act_both(act, g).x; }
+__device__ __forceinline__ float act_slope(int act, float g) { return act_both(act, g).y; }
 
 #define EACH _Pragma("unroll") for (int q = 0; q < NV; ++q) _Pragma("unroll") for (int i = 0; i < 8; ++i)
 
@@ -346,9 +354,9 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
     const int64_t next = after(r);
     if (next < end) fetch(next);
     if (!d.dy) EACH t[q][i] = 0.f;
-    float logit[MODE == EACH1 ? NV : 1][8];
+    float slope[MODE == EACH1 ? NV : 1][8];
     if constexpr (MODE == EACH1) {
-      EACH { logit[q][i] = a[q][i]; a[q][i] = act_fwd(d.gate_act, a[q][i]); }
+      EACH { const float2 as = act_both(d.gate_act, a[q][i]); a[q][i] = as.x; slope[q][i] = as.y; }
     }
     if constexpr (MODE == WHOLE) {
       if (gate != loaded) {
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
         if (MODE == EACH1) {
           T1[q][i] += a[q][i] * tn;
           if (BIAS) T2[BIAS ? q : 0][i] += a[q][i] * ti;
-          logit[MODE == EACH1 ? q : 0][i] = act_slope(d.gate_act, logit[MODE == EACH1 ? q : 0][i]) * (BIAS ? sw[q][i] * tn + sb[BIAS ? q : 0][i] * ti : sw[q][i] * tn);
+          slope[MODE == EACH1 ? q : 0][i] *= (BIAS ? sw[q][i] * tn + sb[BIAS ? q : 0][i] * ti : sw[q][i] * tn);
         } else {
           T1[q][i] += tn;
           if (BIAS) T2[BIAS ? q : 0][i] += ti;
@@ -393,7 +401,7 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
         k1 += t[q][i] * n[q][i];
         if (layer1) k0 += t[q][i];
       }
-      if constexpr (MODE == EACH1) { if (d.dgate) c.template store<FT>(d.dgate, r * d.C, logit); }
+      if constexpr (MODE == EACH1) { if (d.dgate) c.template store<FT>(d.dgate, r * d.C, slope); }
       if (d.df) {
         if (d.post) {
           const float2 s = team.sum2(k1, k0, layer1);
@@ -442,38 +450,51 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
 }
 #undef EACH
 
-// Adds the blocks' column sums: 16 columns x 64 lanes per block, in 64 bits and in a fixed order.  Split gates: lanes_per_gate lanes share
-// the blocks of a gate, the first of them writes dgate and goes on with a T1, a T2.
-template <int FT>
-__global__ __launch_bounds__(1024) void res_norm_finish_kernel(mscl_res_norm_desc d, BwdPlan pl, int lanes_per_gate) {
-  __shared__ double red[4][64][16];
-  const int cl = threadIdx.x & 15, lane = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + cl;
-  const bool in = col < d.C, split = pl.mode == SPLIT && d.gate;
-  const int64_t stride = (int64_t)4 * d.C;
-  const bool want[4] = {d.dh && d.dw_pre, d.dh && d.db_pre, d.f && !split, d.f && !split && d.b_post};
+// Adds the blocks' column sums: COLS columns x 512 / COLS lanes per block, in 64 bits and in a fixed order.  Split gates: lanes_per_gate
+// lanes share the blocks of a gate, the first of them writes dgate and goes on with a T1, a T2.  The launch is latency alone, so a lane
+// has AT_ONCE loads of a sum in flight (out of range: the last row again, times zero), and narrow rows spread over more blocks (COLS 4).
+template <int FT, int COLS>
+__global__ __launch_bounds__(512) void res_norm_finish_kernel(mscl_res_norm_desc d, BwdPlan pl, int lanes_per_gate) {
+  constexpr int AT_ONCE = 8, LANES = 512 / COLS, IN_WAVE = 64 / COLS;
+  __shared__ double red[4][LANES][COLS];
+  const int cl = threadIdx.x % COLS, lane = threadIdx.x / COLS;
+  const int col = blockIdx.x * COLS + cl, C = d.C, at = col < C ? col : C - 1;        // columns past C compute the last one and drop it
+  const bool in = col < C, split = pl.mode == SPLIT && d.gate;
+  const int64_t stride = (int64_t)4 * C;
   double v[4] = {0.0, 0.0, 0.0, 0.0};
-  if (in)
-#pragma unroll 4
-    for (int b = lane; b < pl.blocks; b += 64) {
-      const float* p = d.ws + b * stride + col;
+  // rows first, first + hop, ... below `rows` of sum k
+  auto add = [&](int k, int64_t row0, int first, int hop, int rows) {
+    double s = 0.0;
+    const float* p = d.ws + row0 * stride + (int64_t)k * C + at;
+    for (int b = first; b < rows; b += hop * AT_ONCE) {
+      float x[AT_ONCE];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) if (want[k]) v[k] += (double)p[(int64_t)k * d.C];
+      for (int j = 0; j < AT_ONCE; ++j) { const int e = b + hop * j; x[j] = p[(e < rows ? e : rows - 1) * stride]; }
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) s += b + hop * j < rows ? (double)x[j] : 0.0;
     }
-  const double w = in && d.w_post ? (double)d.w_post[col] : 1.0, b = in && d.b_post ? (double)d.b_post[col] : 0.0;
-  const double s = in && d.scale ? (double)d.scale[col] : 1.0;
-  if (split) {
-    const int at_once = 64 / lanes_per_gate, mine = lane / lanes_per_gate, part = lane % lanes_per_gate;
+    return s;
+  };
+  if (d.dh) {
+    v[0] = add(0, 0, lane, LANES, pl.blocks);
+    if (d.db_pre) v[1] = add(1, 0, lane, LANES, pl.blocks);
+  }
+  const double w = d.w_post ? (double)d.w_post[at] : 1.0, b = d.b_post ? (double)d.b_post[at] : 0.0;
+  const double s = d.scale ? (double)d.scale[at] : 1.0;
+  if (d.f && !split) {
+    v[2] = add(2, 0, lane, LANES, pl.blocks);
+    if (d.b_post) v[3] = add(3, 0, lane, LANES, pl.blocks);
+  } else if (split) {
+    const int at_once = LANES / lanes_per_gate, mine = lane / lanes_per_gate, part = lane % lanes_per_gate;
     for (int g0 = 0; g0 < pl.gates; g0 += at_once) {
       const int g = g0 + mine;
       double s1 = 0.0, s2 = 0.0;
-      if (in && g < pl.gates)
-#pragma unroll 4
-        for (int j = part; j < pl.per_gate; j += lanes_per_gate) {
-          const float* p = d.ws + ((int64_t)g * pl.per_gate + j) * stride + col;
-          s1 += (double)p[2 * (int64_t)d.C];
-          if (d.b_post) s2 += (double)p[3 * (int64_t)d.C];
-        }
+      float logit = 0.f;
+      if (g < pl.gates) {
+        logit = ld1<FT>(d.gate, (int64_t)g * C + at);
+        s1 = add(2, (int64_t)g * pl.per_gate, part, lanes_per_gate, pl.per_gate);
+        if (d.b_post) s2 = add(3, (int64_t)g * pl.per_gate, part, lanes_per_gate, pl.per_gate);
+      }
       if (lanes_per_gate > 1) {
         __syncthreads();
         red[0][lane][cl] = s1;
@@ -482,28 +503,28 @@ __global__ __launch_bounds__(1024) void res_norm_finish_kernel(mscl_res_norm_des
         if (part == 0)
           for (int i = 1; i < lanes_per_gate; ++i) { s1 += red[0][lane + i][cl]; s2 += red[1][lane + i][cl]; }
       }
-      if (part == 0 && in && g < pl.gates) {
-        const float logit = ld1<FT>(d.gate, (int64_t)g * d.C + col), a = act_fwd(d.gate_act, logit);
-        v[2] += (double)a * s1;
-        v[3] += (double)a * s2;
-        if (d.dgate) st1<FT>(d.dgate, (int64_t)g * d.C + col, (float)(s * (double)act_slope(d.gate_act, logit) * (w * s1 + b * s2)));
+      if (part == 0 && g < pl.gates) {
+        const float2 a = act_both(d.gate_act, logit);
+        v[2] += (double)a.x * s1;
+        v[3] += (double)a.x * s2;
+        if (d.dgate && in) st1<FT>(d.dgate, (int64_t)g * C + col, (float)(s * (double)a.y * (w * s1 + b * s2)));
       }
     }
     __syncthreads();
   }
-  // over the 64 lanes of a column: 4 inside a wave, then 16 waves through LDS
+  // over the lanes of a column: those of a wave, then the waves through LDS
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    v[k] += __shfl_xor(v[k], 16, 64);
-    v[k] += __shfl_xor(v[k], 32, 64);
-    if ((lane & 3) == 0) red[k][lane >> 2][cl] = v[k];
+#pragma unroll
+    for (int o = COLS; o < 64; o <<= 1) v[k] += __shfl_xor(v[k], o, 64);
+    if (lane % IN_WAVE == 0) red[k][lane / IN_WAVE][cl] = v[k];
   }
   __syncthreads();
-  if (threadIdx.x >= 16 || !in) return;
+  if (lane != 0 || !in) return;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     v[k] = 0.0;
-    for (int i = 0; i < 16; ++i) v[k] += red[k][i][cl];
+    for (int i = 0; i < 8; ++i) v[k] += red[k][i][cl];
   }
   auto put = [&](float* p, double x) { if (p) p[col] = (float)((d.accumulate ? (double)p[col] : 0.0) + x); };
   if (d.dh) { put(d.dw_pre, v[0]); put(d.db_pre, v[1]); }
@@ -528,8 +549,10 @@ void res_norm_fwd_types(const mscl_res_norm_desc& d, hipStream_t st) {
   int T, wave, nv;
   res_norm_team(d.C, 2, &T, &wave, &nv);
   const int per = wave ? 256 / T : 1;
-  // blocks for 256 CUs of 32 waves; each takes its rows in one stretch
+  // each block takes its rows in one stretch: enough blocks for 32 waves a CU, but no stretch longer than four rows a team -- short enough
+  // that the last blocks end together (32768 x 2048, fp32 / bf16: 172 us with 16 rows a team, 161 with 8, 155 with 4, 158 with 2)
   int64_t grid = wave ? 2048 : 8192 / (T / 64);
+  if (grid < cdiv64(d.rows, 4 * per)) grid = cdiv64(d.rows, 4 * per);
   if (grid > cdiv64(d.rows, per)) grid = cdiv64(d.rows, per);
   const int64_t share = cdiv64(cdiv64(d.rows, grid), per) * per;
   grid = cdiv64(d.rows, share);
@@ -559,9 +582,12 @@ int res_norm_bwd_types(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_
   else if (p.T <= 512) bwd_launch<XT, FT, 1, false, 512>(d, p, st);
   else bwd_launch<XT, FT, 1, false, 1024>(d, p, st);
   MSCL_LAUNCH_CHECK();
+  const int cols = d.C < 1024 ? 4 : 16;
   int lanes = 1;
-  if (d.gate && p.mode == SPLIT) while (lanes * 2 * p.gates <= 64 && lanes * 2 <= p.per_gate) lanes *= 2;
-  hipLaunchKernelGGL(res_norm_finish_kernel<FT>, dim3((d.C + 15) / 16), dim3(1024), 0, st, d, p, lanes);
+  if (d.gate && p.mode == SPLIT) while (lanes * 2 * p.gates <= 512 / cols && lanes * 2 <= p.per_gate) lanes *= 2;
+  const dim3 grid((d.C + cols - 1) / cols);
+  if (cols == 4) hipLaunchKernelGGL((res_norm_finish_kernel<FT, 4>), grid, dim3(512), 0, st, d, p, lanes);
+  else hipLaunchKernelGGL((res_norm_finish_kernel<FT, 16>), grid, dim3(512), 0, st, d, p, lanes);
   MSCL_LAUNCH_CHECK();
   return 0;
 }

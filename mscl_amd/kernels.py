@@ -604,6 +604,10 @@ def _rows_of(t, C):
     return t.contiguous(), C
 
 
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 class ResNormSaved:
     """what res_norm_bwd needs of a forward call"""
     __slots__ = ('x', 'f', 'gate', 'vec', 'stats', 'codes', 'eps', 'shape', 'dims')
@@ -676,13 +680,13 @@ def res_norm_fwd(x, f=None, *, gate=None, gate_act='sigmoid', scale=None, post_n
     stats = [None] * 4                                   # mean_f, rstd_f, mean_y, rstd_y
     if save:
         want = (post_norm == 'layer', post_norm is not None, pre_norm == 'layer', pre_norm is not None)
-        stats = [torch.empty(rows, dtype=torch.float32, device=x.device) if w else None for w in want]
+        held = iter(torch.empty((sum(want), rows), dtype=torch.float32, device=x.device).unbind(0))
+        stats = [next(held) if w else None for w in want]
     if rows:
-        d = lib.ResNormDesc(x=x.data_ptr(), f=ptr(f), gate=ptr(gate), scale=ptr(scale), w_post=ptr(w_post), b_post=ptr(b_post), w_pre=ptr(w_pre),
-                            b_pre=ptr(b_pre), y=ptr(y) if f is not None else None, h=ptr(h), mean_f=ptr(stats[0]), rstd_f=ptr(stats[1]),
-                            mean_y=ptr(stats[2]), rstd_y=ptr(stats[3]), rows=rows, ld_x=ld_x, ld_f=ld_f, rows_per_gate=per, C=C,
-                            x_type=_TYPE_CODE[x.dtype], f_type=_TYPE_CODE[kind], post=NORMS[post_norm], pre=NORMS[pre_norm],
-                            gate_act=GATES[gate_act], eps=eps)
+        d = lib.ResNormDesc(x.data_ptr(), _at(f), _at(gate), _at(scale), _at(w_post), _at(b_post), _at(w_pre), _at(b_pre),
+                            y.data_ptr() if f is not None else None, _at(h), *[_at(t) for t in stats])
+        d.rows, d.ld_x, d.ld_f, d.rows_per_gate, d.C, d.x_type, d.f_type = rows, ld_x, ld_f, per, C, _TYPE_CODE[x.dtype], _TYPE_CODE[kind]
+        d.post, d.pre, d.gate_act, d.eps = NORMS[post_norm], NORMS[pre_norm], GATES[gate_act], eps
         call('mscl_res_norm_fwd', ctypes.byref(d), stream_ptr())
     if not save:
         return y, h, None
@@ -719,23 +723,23 @@ def res_norm_bwd(saved, dy=None, dh=None, into=None, need=None):
     dy = dy.contiguous() if dy is not None else None
     dh = dh.contiguous() if dh is not None else None
     out = {}
+    made = [k for k in names if k in _VECTORS] if into is None else ()
+    if made:                                             # one allocation; zeros where nothing reaches them
+        unreached = rows == 0 or (dh is None and any(k.endswith('pre') for k in made))
+        out = dict(zip(made, (torch.zeros if unreached else torch.empty)((len(made), C), dtype=torch.float32, device=x.device).unbind(0)))
     for k in names:
         if k in _VECTORS:
-            made = k.endswith('pre') and dh is None or rows == 0                 # nothing reaches it
-            out[k] = into[k] if into is not None else (torch.zeros if made else torch.empty)(C, dtype=torch.float32, device=x.device)
+            if into is not None:
+                out[k] = into[k]
         else:
             src = x if k == 'x' else f if k == 'f' else gate
             out[k] = torch.empty(src.shape, dtype=src.dtype, device=x.device)
     if rows == 0:
         return out
-    got = {k: ptr(v) for k, v in out.items()}
-    d = lib.ResNormDesc(x=x.data_ptr(), f=ptr(f), gate=ptr(gate), scale=ptr(vec['scale']), w_post=ptr(vec['w_post']), b_post=ptr(vec['b_post']),
-                        w_pre=ptr(vec['w_pre']), b_pre=ptr(vec['b_pre']), mean_f=ptr(saved.stats[0]), rstd_f=ptr(saved.stats[1]),
-                        mean_y=ptr(saved.stats[2]), rstd_y=ptr(saved.stats[3]), dy=ptr(dy), dh=ptr(dh), dx=got.get('x'), df=got.get('f'),
-                        dgate=got.get('gate'), dscale=got.get('scale'), dw_post=got.get('w_post'), db_post=got.get('b_post'),
-                        dw_pre=got.get('w_pre'), db_pre=got.get('b_pre'), rows=rows, ld_x=ld_x, ld_f=ld_f, rows_per_gate=per, C=C,
-                        x_type=_TYPE_CODE[x.dtype], f_type=_TYPE_CODE[kind], post=post, pre=pre, gate_act=act,
-                        accumulate=int(into is not None), eps=saved.eps)
+    d = lib.ResNormDesc(x.data_ptr(), _at(f), _at(gate), *[_at(vec[k]) for k in _VECTORS], None, None, *[_at(t) for t in saved.stats], _at(dy), _at(dh),
+                        *[_at(out.get(k)) for k in ('x', 'f', 'gate') + _VECTORS])
+    d.rows, d.ld_x, d.ld_f, d.rows_per_gate, d.C, d.x_type, d.f_type = rows, ld_x, ld_f, per, C, _TYPE_CODE[x.dtype], _TYPE_CODE[kind]
+    d.post, d.pre, d.gate_act, d.accumulate, d.eps = post, pre, act, int(into is not None), saved.eps
     n = lib.call_raw('mscl_res_norm_ws', ctypes.byref(d))
     ws = torch.empty(n, dtype=torch.float32, device=x.device)
     d.ws, d.ws_floats = ws.data_ptr(), n

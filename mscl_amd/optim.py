@@ -5,7 +5,7 @@ Three kernels per step (sum of squares, fused clip+decay+momentum+update+bf16 sh
 kernel re-layout for the input-gradient GEMM) instead of ~600 tiny ones.
 
 AdamW (`optimizer=dict(type='AdamW', ...)`, which the reference's build_optimizer hands to torch.optim.AdamW): `AdamW` steps any list of
-GPU tensors in two launches, with moments in 32 or in 8 bits; `ClipAdamW` is the same over a model's arena, beside `ClipSGD`.
+GPU tensors in two or three launches, with moments in 32 or in 8 bits; `ClipAdamW` is the same over a model's arena, beside `ClipSGD`.
 `build_optimizer` picks by the config's `type`."""
 import ctypes
 import math
@@ -98,7 +98,7 @@ class ClipSGD:
         return self._lr.dev
 
 
-BLOCK, CHUNK, PARTS, WORDS = 256, 4096, 256, 32        # = MSCL_ADAMW_* (include/mscl_hip.h)
+BLOCK, CHUNK, PARTS, WORDS = 256, 4096, 2048, 32        # = MSCL_ADAMW_* (include/mscl_hip.h)
 _TYPES = {torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}        # = MSCL_F32 / BF16 / F16
 _TENSOR = np.dtype([('p', '<u8'), ('shadow', '<u8'), ('n', '<i8'), ('off', '<i8'), ('lr_mult', '<f4'), ('decay', '<f4'),
                     ('first_chunk', '<i4'), ('pad', '<i4')])             # = mscl_adamw_tensor
@@ -193,7 +193,7 @@ def _check_args(lr, betas, eps, weight_decay, grad_clip, state_bits, seed=0):
 
 
 class AdamW:
-    """AdamW with decoupled decay over a list of fp32 GPU tensors, two launches per step whatever their number.
+    """AdamW with decoupled decay over a list of fp32 GPU tensors, two or three launches per step whatever their number.
 
     params       fp32 tensors (masters), dense in any dimension order, on one device; no two may share memory
     lr_mult, decay_mult   a factor per tensor on lr / weight_decay (None: 1)
@@ -286,7 +286,6 @@ class AdamW:
             self._grad_ptrs = ptrs
         self._desc.grad_type = _TYPES[grads[0].dtype]
 
-    @torch.no_grad()
     def step(self, grads=None):
         if torch.cuda.current_device() != self.device.index:
             with torch.cuda.device(self.device):
@@ -315,10 +314,12 @@ class AdamW:
         """(exp_avg, exp_avg_sq) as numbers, flat: the fp32 states themselves, or what the 8-bit codes stand for, in bf16 (exact)"""
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
-        m, v = (torch.empty(self.numel, dtype=torch.bfloat16, device=self.device) for _ in range(2))
-        with torch.cuda.device(self.device):
-            lib.call('mscl_adamw_values', lib.ptr(self.exp_avg), lib.ptr(self.exp_avg_sq), lib.ptr(self.exponents), lib.ptr(m), lib.ptr(v),
-                     self.numel // BLOCK, lib.stream_ptr())
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.state_values()
+        m, v = torch.empty((2, self.numel), dtype=torch.bfloat16, device=self.device).unbind(0)
+        lib.call('mscl_adamw_values', self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.exponents.data_ptr(), m.data_ptr(), v.data_ptr(),
+                 self.numel // BLOCK, lib.stream_ptr())
         return m, v
 
     def device_step(self):
