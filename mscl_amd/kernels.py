@@ -608,6 +608,11 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+def _empty(t, dtype):
+    """a dense tensor of t's shape (empty_like is half the host time of empty, but keeps a permuted layout)"""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else torch.empty(t.shape, dtype=dtype, device=t.device)
+
+
 class ResNormSaved:
     """what res_norm_bwd needs of a forward call"""
     __slots__ = ('x', 'f', 'gate', 'vec', 'stats', 'codes', 'eps', 'shape', 'dims')
@@ -632,25 +637,25 @@ def _res_norm_check(x, f, gate, vec, post_norm, pre_norm, gate_act, eps):
         raise lib.MsclError(f'res_norm: fp32, bf16 or fp16, equal for x and f or x in fp32; got {x.dtype}, {kind}')
     if f is not None and f.shape != x.shape:
         raise lib.MsclError(f'res_norm: f {tuple(f.shape)} does not fit x {tuple(x.shape)}')
+    dev = x.device
     for k, v in vec.items():
         if v is None:
             continue
-        if v.dtype != torch.float32 or tuple(v.shape) != (C,) or not v.is_contiguous() or v.device != x.device:
+        if v.dtype is not torch.float32 or v.dim() != 1 or v.shape[0] != C or not v.is_contiguous() or v.device != dev:
             raise lib.MsclError(f'res_norm: {k} is a contiguous fp32 vector of {C} channels beside x')
-        if (k.endswith('post') and post_norm is None) or (k.endswith('pre') and pre_norm is None):
+        if k != 'scale' and (post_norm if k[2:] == 'post' else pre_norm) is None:
             raise lib.MsclError(f'res_norm: {k} without its norm')
     per = 0
     if gate is not None:
         whole = gate.shape == x.shape
-        if gate.dtype != kind or gate.device != x.device or not (whole or (gate.dim() == 2 and gate.shape[1] == C)):
+        if gate.dtype != kind or gate.device != dev or not (whole or (gate.dim() == 2 and gate.shape[1] == C)):
             raise lib.MsclError(f"res_norm: gate is (gates, {C}) or like x, of f's type; got {tuple(gate.shape)} {gate.dtype}")
         n = gate.numel() // C
         if rows and (n == 0 or rows % n):
             raise lib.MsclError(f'res_norm: {n} gates do not divide {rows} rows')
         per = rows // n if n else 0
-    for t in (f, gate):
-        if t is not None and t.device != x.device:
-            raise lib.MsclError('res_norm: all tensors on one device')
+    if f is not None and f.device != dev:
+        raise lib.MsclError('res_norm: all tensors on one device')
     return rows, C, per
 
 
@@ -673,11 +678,11 @@ def res_norm_fwd(x, f=None, *, gate=None, gate_act='sigmoid', scale=None, post_n
     if f is not None:
         kind = f.dtype
         f, ld_f = _rows_of(f, C)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = _empty(x, x.dtype)
     if gate is not None:
         gate = gate.contiguous()
-    h = torch.empty(x.shape, dtype=kind, device=x.device) if pre_norm is not None else None
-    stats = [None] * 4                                   # mean_f, rstd_f, mean_y, rstd_y
+    h = _empty(x, kind) if pre_norm is not None else None
+    stats = (None,) * 4                                  # mean_f, rstd_f, mean_y, rstd_y
     if save:
         want = (post_norm == 'layer', post_norm is not None, pre_norm == 'layer', pre_norm is not None)
         held = iter(torch.empty((sum(want), rows), dtype=torch.float32, device=x.device).unbind(0))
@@ -733,7 +738,7 @@ def res_norm_bwd(saved, dy=None, dh=None, into=None, need=None):
                 out[k] = into[k]
         else:
             src = x if k == 'x' else f if k == 'f' else gate
-            out[k] = torch.empty(src.shape, dtype=src.dtype, device=x.device)
+            out[k] = _empty(src, src.dtype)
     if rows == 0:
         return out
     d = lib.ResNormDesc(x.data_ptr(), _at(f), _at(gate), *[_at(vec[k]) for k in _VECTORS], None, None, *[_at(t) for t in saved.stats], _at(dy), _at(dh),

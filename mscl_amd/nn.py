@@ -962,3 +962,80 @@ class Conv1dK1Hip(nn.Module):
         self.weight = nn.Parameter(ref.weight.detach().clone())
         self.bias = nn.Parameter(ref.bias.detach().clone())
         self._rt = None
+
+
+# ------------------------------------------------------------------------------------------ residual norm
+class _ResNormFn(torch.autograd.Function):
+    """(y, h) of kernels.res_norm_fwd as one graph node; h alone without a branch.  The module's own gradients go straight into the arena."""
+
+    @staticmethod
+    def forward(ctx, x, f, gate, anchor, mod):
+        y, h, saved = K.res_norm_fwd(x, f, gate=gate, save=True, **mod._args(f is not None))
+        tensors = [t for t in (saved.x, saved.f, saved.gate) if t is not None]
+        ctx.save_for_backward(*tensors)                  # (its version check refuses a backward over inputs changed in place)
+        ctx.saved, ctx.mod = saved, mod
+        ctx.capturing = torch.cuda.is_current_stream_capturing()
+        ctx.set_materialize_grads(False)
+        return h if f is None else y if h is None else (y, h)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        ctx.saved_tensors
+        if torch.cuda.is_current_stream_capturing() != ctx.capturing:
+            raise MsclError('residual norm: forward and backward belong into the same graph capture, or both outside of one')
+        saved, mod = ctx.saved, ctx.mod
+        if saved.f is None:
+            dy, dh = None, grads[0]
+        else:
+            dy, dh = grads if mod.pre is not None else (grads[0], None)
+        if dy is None and dh is None:
+            return None, None, None, None, None
+        need = [k for k, w in zip(('x', 'f', 'gate'), ctx.needs_input_grad) if w] + list(mod._live(saved.f is not None, dh is not None))
+        out = K.res_norm_bwd(saved, dy, dh, into=mod._rt['grad'], need=need)
+        for k in mod._live(saved.f is not None, dh is not None):
+            mod._rt['slots'][k].touched = True
+        return out.get('x'), out.get('f'), out.get('gate'), None, None
+
+
+class ResNormHip(nn.Module):
+    """What stands between two residual blocks on NDHWC rows, `y = x + scale * act(gate) * norm_post(f)` and the next block's input
+    `h = norm_pre(y)`, in one pass each way (kernels.res_norm_fwd / _bwd) -- the counterpart of BatchNorm + residual where statistics are
+    taken over a position's channels.  post, pre: 'rms', 'layer' or None; scale: initial residual scale per channel (None: none);
+    bias: norms with biases; gates are passed to forward.  Bound to a model's arena by materialize(), like every module here."""
+    is_norm = True                       # its parameters follow norm_decay_mult (optim.ClipAdamW)
+
+    def __init__(self, channels, post='rms', pre='rms', scale=None, bias=False, gate_act='sigmoid', eps=1e-6):
+        super().__init__()
+        if post not in K.NORMS or pre not in K.NORMS or gate_act not in K.GATES:
+            raise ValueError(f'norms are rms, layer or None, gates linear, sigmoid or tanh; got {post}, {pre}, {gate_act}')
+        self.channels, self.post, self.pre, self.gate_act, self.eps = channels, post, pre, gate_act, eps
+        fill = dict(scale=scale, w_post=1.0 if post else None, b_post=0.0 if post and bias else None, w_pre=1.0 if pre else None,
+                    b_pre=0.0 if pre and bias else None)
+        for name, v in fill.items():
+            self.register_parameter(name, None if v is None else nn.Parameter(torch.full((channels,), float(v))))
+        self._rt = self._anchor = None
+
+    def extra_repr(self):
+        return f'{self.channels}, post={self.post}, pre={self.pre}, gate_act={self.gate_act}, eps={self.eps}'
+
+    def _args(self, branch):
+        vec = self._rt['vec']
+        if not branch:
+            return dict(pre_norm=self.pre, w_pre=vec['w_pre'], b_pre=vec['b_pre'], eps=self.eps)
+        return dict(vec, post_norm=self.post, pre_norm=self.pre, gate_act=self.gate_act, eps=self.eps)
+
+    def _live(self, branch, dh):
+        """the parameters that a backward pass reaches"""
+        return [k for k in self._rt['slots'] if (dh if k.endswith('pre') else branch)]
+
+    def forward(self, x, f=None, gate=None):
+        """(y, h); without a branch f the input norm of a first block: (x, norm_pre(x))"""
+        if self._rt is None:
+            raise MsclError('call materialize("cuda") on the model first')
+        if not torch.is_grad_enabled():
+            y, h, _ = K.res_norm_fwd(x, f, gate=gate, **self._args(f is not None))
+            return y, h
+        if self._anchor is None or self._anchor.device != x.device:
+            self._anchor = torch.zeros(1, device=x.device, requires_grad=True)
+        out = _ResNormFn.apply(x, f, gate, self._anchor, self)
+        return (x, out) if f is None else out if self.pre is not None else (out, None)

@@ -111,6 +111,10 @@ def bind_module(m, ar, key, rec):
         shp = (m.out_channels, m.in_channels)
         m._rt = dict(w=ar.view(P, sw).view(shp), b=ar.view(P, sb), slot_w=sw, slot_b=sb,
                      dw=ar.view('G', sw).view(shp), db=ar.view('G', sb))
+    elif isinstance(m, nn_hip.ResNormHip):
+        slots = {n: p._mscl_slot for n, p in m.named_parameters(recurse=False)}
+        m._rt = dict(slots=slots, vec={n: ar.view(P, slots[n]) if n in slots else None for n in K._VECTORS},
+                     grad=None if key else {n: ar.view('G', s) for n, s in slots.items()})
 
 
 @RECOGNIZERS.register_module()
