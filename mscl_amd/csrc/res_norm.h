@@ -16,7 +16,7 @@
 // A TEAM of lanes owns a row: 1 .. 16 or 64 lanes of a wave (sums by DPP), or the whole block (sums through LDS).  A lane holds NV x 8
 // adjacent channels in registers, so a row is read once; the loads of a team's next row are in flight while it works on the current one.
 // Accesses are 16 bytes at the alignment of an element (the memory path of gfx950 takes any), so odd widths and strides run the same
-// code; only the lane with the last, partial 8 channels goes element by element.
+// code.
 #include "common.h"
 #include <hip/hip_fp16.h>
 
@@ -48,32 +48,38 @@ template <int T> __device__ __forceinline__ void unpack(const Raw<T>& u, float* 
   }
 }
 
-// a lane's channels of a row: value (q, i) is channel (q T + lane) 8 + i
-template <int NV> struct Cols {
-  int lane, T, C;
-  __device__ __forceinline__ int col(int q) const { return (q * T + lane) * 8; }
-  __device__ __forceinline__ int count(int q) const { const int n = C - col(q); return n < 0 ? 0 : n; }        // 8 or more: all
-  // channels past C read as zero
+// A lane's channels of a row: value (q, i) is channel col[q] + i, 8 adjacent ones.  The last vector of a row that is no multiple of 8 wide
+// ends with the row, and so repeats up to 7 channels of the vector before it: both lanes compute -- and store -- the same bits for
+// them, and the first `skip` values of the later one stay out of the row's sums.  A lane past the row repeats the last vector, skips all
+// 8 and stores nothing.  So every load is one unconditional access of 16 (32) bytes.  NARROW: rows of fewer than 8 channels have
+// their values at the end of one vector and go element by element.
+template <int NV, bool NARROW> struct Cols {
+  int col[NV], skip[NV];
+  __device__ __forceinline__ Cols(int lane, int T, int C) {
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      const int at = (q * T + lane) * 8;
+      skip[q] = at >= C ? 8 : at + 8 > C ? at + 8 - C : 0;
+      col[q] = at + 8 > C ? C - 8 : at;
+    }
+  }
   template <int TY> __device__ __forceinline__ void fetch(const void* p, int64_t row, Raw<TY> (&u)[NV]) const {
     constexpr int sz = TY == MSCL_F32 ? 4 : 2;
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-      const char* a = (const char*)p + (row + col(q)) * sz;
-      const int n = count(q);
-      if (n >= 8) {
+      const char* a = (const char*)p + (row + col[q]) * sz;
+      if (!NARROW) {
         if (TY == MSCL_F32) __builtin_memcpy(u[q].w, (const float*)a, 32);
         else __builtin_memcpy(u[q].w, (const uint16_t*)a, 16);
       } else {
 #pragma unroll
         for (int i = 0; i < (TY == MSCL_F32 ? 8 : 4); ++i) u[q].w[i] = 0;
-        if (n > 0) {
 #pragma unroll
-          for (int i = 0; i < 7; ++i)
-            if (i < n) {
-              if (TY == MSCL_F32) u[q].w[i] = ((const uint32_t*)a)[i];
-              else u[q].w[i >> 1] |= (uint32_t)((const uint16_t*)a)[i] << (16 * (i & 1));
-            }
-        }
+        for (int i = 1; i < 8; ++i)
+          if (i >= skip[q]) {
+            if (TY == MSCL_F32) u[q].w[i] = ((const uint32_t*)a)[i];
+            else u[q].w[i >> 1] |= (uint32_t)((const uint16_t*)a)[i] << (16 * (i & 1));
+          }
       }
     }
   }
@@ -83,22 +89,22 @@ template <int NV> struct Cols {
 #pragma unroll
     for (int q = 0; q < NV; ++q) unpack<TY>(u[q], v[q]);
   }
-  // a per-channel vector; a missing one is all `one`.  Zero past C, so that those channels add nothing to a row's sums
+  // a per-channel vector; a missing one is all `one`
   __device__ __forceinline__ void load_vec(const float* p, float one, float (&v)[NV][8]) const {
     if (p) load<MSCL_F32>(p, 0, v);
     else
 #pragma unroll
       for (int q = 0; q < NV; ++q)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[q][i] = i < count(q) ? one : 0.f;
+        for (int i = 0; i < 8; ++i) v[q][i] = one;
   }
   template <int TY> __device__ __forceinline__ void store(void* p, int64_t row, const float (&v)[NV][8]) const {
     constexpr int sz = TY == MSCL_F32 ? 4 : 2;
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-      char* a = (char*)p + (row + col(q)) * sz;
-      const int n = count(q);
-      if (n >= 8) {
+      char* a = (char*)p + (row + col[q]) * sz;
+      if (skip[q] == 8) continue;
+      if (!NARROW) {
         if (TY == MSCL_F32) __builtin_memcpy((float*)a, v[q], 32);
         else {
           uint32_t w[4];
@@ -107,15 +113,32 @@ template <int NV> struct Cols {
             w[i] = TY == MSCL_BF16 ? pack2bf(v[q][2 * i], v[q][2 * i + 1]) : (uint32_t)f2h(v[q][2 * i]) | (uint32_t)f2h(v[q][2 * i + 1]) << 16;
           __builtin_memcpy((uint16_t*)a, w, 16);
         }
-      } else if (n > 0) {
+      } else {
 #pragma unroll
-        for (int i = 0; i < 7; ++i) if (i < n) st1<TY>(a, i, v[q][i]);
+        for (int i = 1; i < 8; ++i) if (i >= skip[q]) st1<TY>(a, i, v[q][i]);
       }
     }
   }
+  // sum of f(q, i) over the lane's own channels
+  template <class F> __device__ __forceinline__ float sum(F f) const {
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t += f(q, i);
+      if (skip[q]) {
+        t = 0.f;
+#pragma unroll
+        for (int i = 1; i < 8; ++i) t += i >= skip[q] ? f(q, i) : 0.f;
+      }
+      s += t;
+    }
+    return s;
+  }
 };
 
-// team sums.  WAVE: T in {1, 2, 4, 8, 16, 64}.  Block teams: waves meet in LDS; two alternating slots make one barrier per sum enough
+// team sums.  WAVE: T in {1, 2, 4, 8, 16, 32, 64}.  Block teams: waves meet in LDS; two alternating slots make one barrier per sum enough
 // (a slot is written again only by waves that have passed the barrier of the sum between, i.e. after every wave has read it).
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
   return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
@@ -130,6 +153,10 @@ template <bool WAVE> struct Team {
     if (T >= 4) v = dpp_add<0x4E>(v);        // quad_perm: other pair
     if (T >= 8) v = dpp_add<0x141>(v);       // row_half_mirror: other quad
     if (T >= 16) v = dpp_add<0x128>(v);      // row_ror 8: other half row
+    if (T == 32) {                           // the rows of a pair: {r0, r0, r2, r2} + {r1, r1, r3, r3}
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
     return v;
   }
   __device__ __forceinline__ float2 sum2(float a, float b, bool want_b) {
@@ -166,102 +193,116 @@ __device__ __forceinline__ float2 act_both(int act, float g) {
   }
   return make_float2(g, 1.f);
 }
-__device__ __forceinline__ float act_fwd(int act, float g) { return act_both(act, g).x; }
-__device__ __forceinline__ float act_slope(int act, float g) { return act_both(act, g).y; }
+// the values (and slopes) of a lane's gates, one branch for all of them
+template <bool SLOPE, int NV>
+__device__ __forceinline__ void act_row(int act, float (&a)[NV][8], float (*slope)[8]) {
+  auto each = [&](int kind) {
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 v = act_both(kind, a[q][i]);
+        a[q][i] = v.x;
+        if (SLOPE) slope[q][i] = v.y;
+      }
+  };
+  if (act == MSCL_GATE_SIGMOID) each(MSCL_GATE_SIGMOID);
+  else if (act == MSCL_GATE_TANH) each(MSCL_GATE_TANH);
+  else each(MSCL_GATE_LINEAR);
+}
 
 #define EACH _Pragma("unroll") for (int q = 0; q < NV; ++q) _Pragma("unroll") for (int i = 0; i < 8; ++i)
 
 // mean and 1 / deviation of a row held in v (rms: mean 0); the second moment is taken about the mean, in a second pass over registers
-template <int NV, bool WAVE>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], int kind, float inv_c, float eps, const Cols<NV>& c, Team<WAVE>& team) {
-  float mu = 0.f, s = 0.f;
-  if (kind == MSCL_NORM_LAYER) {
-    EACH s += v[q][i];              // channels past C are zero
-    mu = team.sum(s) * inv_c;
-    s = 0.f;
-    EACH { const float d = i < c.count(q) ? v[q][i] - mu : 0.f; s += d * d; }
-  } else {
-    EACH s += v[q][i] * v[q][i];
-  }
+template <int NV, bool WAVE, class C>
+__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], int kind, float inv_c, float eps, const C& c, Team<WAVE>& team) {
+  float mu = 0.f;
+  if (kind == MSCL_NORM_LAYER) mu = team.sum(c.sum([&](int q, int i) { return v[q][i]; })) * inv_c;
+  const float s = c.sum([&](int q, int i) { const float d = v[q][i] - mu; return d * d; });
   return make_float2(mu, 1.f / sqrtf(team.sum(s) * inv_c + eps));
 }
 }  // namespace
 
 // A block takes `share` consecutive rows, its teams in turn.  EACH_GATE: a gate for every row, fetched with it; otherwise the gate's
 // activation stays in registers until a row belongs to another gate.  BIAS: b_post or b_pre present.
-template <int XT, int FT, int NV, bool WAVE, bool EACH_GATE, bool BIAS>
+template <int XT, int FT, int NV, bool WAVE, bool EACH_GATE, bool BIAS, bool NARROW>
 __global__ __launch_bounds__(WAVE ? 256 : 1024) void res_norm_fwd_kernel(mscl_res_norm_desc d, int T, FastDiv gdiv, int64_t share) {
   __shared__ float2 red[32];
   Team<WAVE> team{T, red, 0};
   const int per = WAVE ? 256 / T : 1, sub = WAVE ? (int)threadIdx.x / T : 0;
-  const Cols<NV> c{WAVE ? (int)threadIdx.x % T : (int)threadIdx.x, T, d.C};
+  const int lane = WAVE ? (int)threadIdx.x % T : (int)threadIdx.x;
+  const Cols<NV, NARROW> c(lane, T, d.C);
   const float inv_c = 1.f / (float)d.C;
   const int64_t end = share * (blockIdx.x + 1) < d.rows ? share * (blockIdx.x + 1) : d.rows;
   int64_t r = share * blockIdx.x + sub;
   Raw<XT> ux[NV];
   Raw<FT> uf[NV], ug[NV];
-  if (r < end) {
-    c.template fetch<XT>(d.x, r * d.ld_x, ux);
-    if (d.f) c.template fetch<FT>(d.f, r * d.ld_f, uf);
-    if (EACH_GATE) c.template fetch<FT>(d.gate, r * d.C, ug);
-  }
+  constexpr bool LEAN = NV > 1 && !WAVE;
+  auto fetch = [&](int64_t at) {
+    c.template fetch<XT>(d.x, at * d.ld_x, ux);
+    if (d.f) c.template fetch<FT>(d.f, at * d.ld_f, uf);
+    if (EACH_GATE) c.template fetch<FT>(d.gate, at * d.C, ug);
+  };
+  if (!LEAN && r < end) fetch(r);
   float sw[NV][8], sb[BIAS ? NV : 1][8], w2[NV][8], b2[BIAS ? NV : 1][8], a[NV][8];
-  if (d.f) {
-    c.load_vec(d.scale, 1.f, a);
+  auto post_vectors = [&] {
+    float s[NV][8];
+    c.load_vec(d.scale, 1.f, s);
     c.load_vec(d.w_post, 1.f, sw);
-    EACH sw[q][i] *= a[q][i];
+    EACH sw[q][i] *= s[q][i];
     if constexpr (BIAS) {
       c.load_vec(d.b_post, 0.f, sb);
-      EACH sb[q][i] *= a[q][i];
+      EACH sb[q][i] *= s[q][i];
     }
-    EACH a[q][i] = 1.f;
-  }
-  if (d.pre) {
+  };
+  auto pre_vectors = [&] {
     c.load_vec(d.w_pre, 1.f, w2);
     if constexpr (BIAS) c.load_vec(d.b_pre, 0.f, b2);
-  }
+  };
+  if (!LEAN && d.f) post_vectors();
+  if (!LEAN && d.pre) pre_vectors();
+  EACH a[q][i] = 1.f;
   int gate = -1;
   for (; r < end; r += per) {
     float x[NV][8], f[NV][8];
+    if (LEAN) fetch(r);
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       unpack<XT>(ux[q], x[q]);
       if (d.f) unpack<FT>(uf[q], f[q]);
       if (EACH_GATE) unpack<FT>(ug[q], a[q]);
     }
-    if (r + per < end) {
-      c.template fetch<XT>(d.x, (r + per) * d.ld_x, ux);
-      if (d.f) c.template fetch<FT>(d.f, (r + per) * d.ld_f, uf);
-      if (EACH_GATE) c.template fetch<FT>(d.gate, (r + per) * d.C, ug);
-    }
+    if (!LEAN && r + per < end) fetch(r + per);
     if (d.f) {
       if (EACH_GATE) {
-        EACH a[q][i] = act_fwd(d.gate_act, a[q][i]);
+        act_row<false, NV>(d.gate_act, a, nullptr);
       } else if (d.gate) {
         const int g = fdiv((int)r, gdiv);
         if (g != gate) {
           gate = g;
           c.template load<FT>(d.gate, (int64_t)g * d.C, a);
-          EACH a[q][i] = act_fwd(d.gate_act, a[q][i]);
+          act_row<false, NV>(d.gate_act, a, nullptr);
         }
       }
       if (d.post) {
         const float2 st = row_stats<NV, WAVE>(f, d.post, inv_c, d.eps, c, team);
-        if (c.lane == 0) {
+        if (lane == 0) {
           if (d.mean_f) d.mean_f[r] = st.x;
           if (d.rstd_f) d.rstd_f[r] = st.y;
         }
         EACH f[q][i] = (f[q][i] - st.x) * st.y;
       }
-      EACH x[q][i] += a[q][i] * (BIAS ? sw[q][i] * f[q][i] + sb[BIAS ? q : 0][i] : sw[q][i] * f[q][i]);       // zero past C: sw, sb are
+      if (LEAN) post_vectors();
+      EACH x[q][i] += a[q][i] * (BIAS ? sw[q][i] * f[q][i] + sb[BIAS ? q : 0][i] : sw[q][i] * f[q][i]);
       c.template store<XT>(d.y, r * d.C, x);
     }
     if (d.pre) {
       const float2 st = row_stats<NV, WAVE>(x, d.pre, inv_c, d.eps, c, team);
-      if (c.lane == 0) {
+      if (lane == 0) {
         if (d.mean_y) d.mean_y[r] = st.x;
         if (d.rstd_y) d.rstd_y[r] = st.y;
       }
+      if (LEAN) pre_vectors();
       EACH { x[q][i] = (x[q][i] - st.x) * st.y * w2[q][i]; if (BIAS) x[q][i] += b2[BIAS ? q : 0][i]; }
       c.template store<FT>(d.h, r * d.C, x);
     }
@@ -276,15 +317,20 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void res_norm_fwd_kernel(mscl_re
 enum { SPLIT = 0, WHOLE = 1, EACH1 = 2 };
 struct BwdPlan { int T, wave, nv, mode, per_gate, gates, blocks, rows_per_gate; };
 
-template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS>
-__global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_desc d, BwdPlan pl) {
+// Waves a SIMD asked of the compiler: 4 (128 registers a lane) where that costs next to no spills, 3 for the forms with more sums; a gate per
+// element without biases runs best at what it takes by itself (11712 x 2048: 144 us of a training pass, 153 at 3, 180 at 4).
+// LEAN (past 8192 channels, 16 of them a lane, 1024 lanes): no prefetch, the per-channel vectors read again for every row -- registers.
+constexpr int bwd_waves(int mode, bool bias) { return mode == SPLIT && !bias ? 4 : mode == EACH1 && !bias ? 1 : 3; }
+template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS, bool NARROW>
+__global__ __launch_bounds__(THREADS, THREADS > 512 ? THREADS / 256 : bwd_waves(MODE, BIAS)) void res_norm_bwd_kernel(mscl_res_norm_desc d, BwdPlan pl) {
   extern __shared__ float lds[];                    // wave teams: [256][8 NV] for the column sums of a block
   __shared__ float2 red[32];
   constexpr int NB = BIAS ? NV : 1;
   const int T = pl.T;
   Team<WAVE> team{T, red, 0};
   const int per = WAVE ? 256 / T : 1, sub = WAVE ? (int)threadIdx.x / T : 0;
-  const Cols<NV> c{WAVE ? (int)threadIdx.x % T : (int)threadIdx.x, T, d.C};
+  const int lane = WAVE ? (int)threadIdx.x % T : (int)threadIdx.x;
+  const Cols<NV, NARROW> c(lane, T, d.C);
   const float inv_c = 1.f / (float)d.C;
   const bool layer2 = d.pre == MSCL_NORM_LAYER, layer1 = d.post == MSCL_NORM_LAYER;
 
@@ -319,29 +365,35 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
     if (d.f && d.post) { if (layer1) sd[0] = d.mean_f[at]; sd[1] = d.rstd_f[at]; }
     if (d.dh) { if (layer2) sd[2] = d.mean_y[at]; sd[3] = d.rstd_y[at]; }
   };
-  if (r < end) fetch(r);
+  constexpr bool LEAN = NV > 1;
+  if (!LEAN && r < end) fetch(r);
 
   float sw[NV][8], sb[NB][8], w2[NV][8], a[NV][8];
   float U1[NV][8] = {}, U2[NB][8] = {}, T1[NV][8] = {}, T2[NB][8] = {}, t1[MODE == WHOLE ? NV : 1][8] = {}, t2[MODE == WHOLE ? NB : 1][8] = {};
-  if (d.f) {
-    c.load_vec(d.scale, 1.f, a);
-    c.load_vec(d.w_post, 1.f, sw);
-    EACH sw[q][i] *= a[q][i];
-    if constexpr (BIAS) {
-      c.load_vec(d.b_post, 0.f, sb);
-      EACH sb[q][i] *= a[q][i];
+  auto vectors = [&] {
+    if (d.f) {
+      float s[NV][8];
+      c.load_vec(d.scale, 1.f, s);
+      c.load_vec(d.w_post, 1.f, sw);
+      EACH sw[q][i] *= s[q][i];
+      if constexpr (BIAS) {
+        c.load_vec(d.b_post, 0.f, sb);
+        EACH sb[q][i] *= s[q][i];
+      }
     }
-    EACH a[q][i] = 1.f;
-  }
-  if (d.dh) c.load_vec(d.w_pre, 1.f, w2);
+    if (d.dh) c.load_vec(d.w_pre, 1.f, w2);
+  };
+  if (!LEAN) vectors();
+  EACH a[q][i] = 1.f;
   if (MODE == SPLIT && d.gate) {
     c.template load<FT>(d.gate, gate * d.C, a);
-    EACH a[q][i] = act_fwd(d.gate_act, a[q][i]);
+    act_row<false, NV>(d.gate_act, a, nullptr);
   }
   int64_t loaded = -1;
 
   while (r < end) {
     float x[NV][8], n[NV][8], t[NV][8], g[NV][8];
+    if (LEAN) { fetch(r); vectors(); }
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       unpack<XT>(ux[q], x[q]);
@@ -352,17 +404,17 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
     }
     const float mu1 = sd[0], r1 = sd[1], mu2 = sd[2], r2 = sd[3];
     const int64_t next = after(r);
-    if (next < end) fetch(next);
+    if (!LEAN && next < end) fetch(next);
     if (!d.dy) EACH t[q][i] = 0.f;
     float slope[MODE == EACH1 ? NV : 1][8];
     if constexpr (MODE == EACH1) {
-      EACH { const float2 as = act_both(d.gate_act, a[q][i]); a[q][i] = as.x; slope[q][i] = as.y; }
+      act_row<true, NV>(d.gate_act, a, slope);
     }
     if constexpr (MODE == WHOLE) {
       if (gate != loaded) {
         loaded = gate;
         c.template load<FT>(d.gate, gate * d.C, a);
-        EACH a[q][i] = act_fwd(d.gate_act, a[q][i]);
+        act_row<false, NV>(d.gate_act, a, nullptr);
       }
     }
     if (d.f) {
@@ -370,23 +422,21 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
       if (d.dh) EACH x[q][i] += a[q][i] * (BIAS ? sw[q][i] * n[q][i] + sb[BIAS ? q : 0][i] : sw[q][i] * n[q][i]);        // y
     }
     if (d.dh) {
-      float c1 = 0.f, c0 = 0.f;
       EACH {
-        const float yh = (x[q][i] - mu2) * r2;      // past C: dh and w2 are zero, nothing of yh reaches a sum
+        const float yh = (x[q][i] - mu2) * r2;
         x[q][i] = yh;
         U1[q][i] += g[q][i] * yh;
         if (BIAS) U2[BIAS ? q : 0][i] += g[q][i];
         g[q][i] *= w2[q][i];
-        c1 += g[q][i] * yh;
-        if (layer2) c0 += g[q][i];
       }
+      const float c1 = c.sum([&](int q, int i) { return g[q][i] * x[q][i]; });
+      const float c0 = layer2 ? c.sum([&](int q, int i) { return g[q][i]; }) : 0.f;
       const float2 s = team.sum2(c1, c0, layer2);
       const float m1 = s.x * inv_c, m0 = s.y * inv_c;
       EACH t[q][i] += r2 * (g[q][i] - m0 - x[q][i] * m1);
     }
     if (d.dx) c.template store<XT>(d.dx, r * d.C, t);
     if (d.f) {
-      float k1 = 0.f, k0 = 0.f;
       EACH {
         const float ti = t[q][i], tn = ti * n[q][i];
         if (MODE == EACH1) {
@@ -397,13 +447,13 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
           T1[q][i] += tn;
           if (BIAS) T2[BIAS ? q : 0][i] += ti;
         }
-        t[q][i] = ti * a[q][i] * sw[q][i];          // zero past C: sw is
-        k1 += t[q][i] * n[q][i];
-        if (layer1) k0 += t[q][i];
+        t[q][i] = ti * a[q][i] * sw[q][i];
       }
       if constexpr (MODE == EACH1) { if (d.dgate) c.template store<FT>(d.dgate, r * d.C, slope); }
       if (d.df) {
         if (d.post) {
+          const float k1 = c.sum([&](int q, int i) { return t[q][i] * n[q][i]; });
+          const float k0 = layer1 ? c.sum([&](int q, int i) { return t[q][i]; }) : 0.f;
           const float2 s = team.sum2(k1, k0, layer1);
           const float m1 = s.x * inv_c, m0 = s.y * inv_c;
           EACH t[q][i] = r1 * (t[q][i] - m0 - n[q][i] * m1);
@@ -413,12 +463,13 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
       if constexpr (MODE == WHOLE) {
         if (next != r + 1 || next >= end || pl.rows_per_gate == 1) {        // the gate's last row
           c.template load<FT>(d.gate, gate * d.C, x);
+          act_row<true, NV>(d.gate_act, x, n);
           EACH {
             const float s1 = T1[q][i], s2 = BIAS ? T2[BIAS ? q : 0][i] : 0.f;
             t1[q][i] += a[q][i] * s1;
             T1[q][i] = 0.f;
             if (BIAS) { t2[BIAS ? q : 0][i] += a[q][i] * s2; T2[BIAS ? q : 0][i] = 0.f; }
-            x[q][i] = act_slope(d.gate_act, x[q][i]) * (BIAS ? sw[q][i] * s1 + sb[BIAS ? q : 0][i] * s2 : sw[q][i] * s1);
+            x[q][i] = n[q][i] * (BIAS ? sw[q][i] * s1 + sb[BIAS ? q : 0][i] * s2 : sw[q][i] * s1);
           }
           if (d.dgate) c.template store<FT>(d.dgate, gate * d.C, x);
           gate += step;
@@ -439,7 +490,7 @@ __global__ __launch_bounds__(THREADS) void res_norm_bwd_kernel(mscl_res_norm_des
                  : (MODE == WHOLE ? t2[MODE == WHOLE && BIAS ? q : 0][i] : T2[BIAS ? q : 0][i]);
     if (!WAVE) { c.template store<MSCL_F32>(out + (int64_t)k * d.C, 0, v); continue; }
     __syncthreads();
-    EACH lds[sub * T * 8 * NV + c.col(q) + i] = v[q][i];
+    EACH if (i >= c.skip[q]) lds[sub * T * 8 * NV + c.col[q] + i] = v[q][i];
     __syncthreads();
     for (int e = threadIdx.x; e < d.C; e += 256) {
       float s = 0.f;
@@ -534,15 +585,23 @@ __global__ __launch_bounds__(512) void res_norm_finish_kernel(mscl_res_norm_desc
 // ---------------------------------------------------------------------------------------------------------------- launches
 // lanes, kind of team and channels per lane for rows of C channels (res_norm.hip)
 void res_norm_team(int C, int max_wave_nv, int* T, int* wave, int* nv);
+template <int XT, int FT, int NV, bool WAVE, bool EACH, bool BIAS, bool NARROW = false>
+static void fwd_go(const mscl_res_norm_desc& d, int T, unsigned grid, int64_t share, hipStream_t st) {
+  const FastDiv g = make_fastdiv(d.gate ? (int)d.rows_per_gate : 1);
+  hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, EACH, BIAS, NARROW>), dim3(grid), dim3(WAVE ? 256 : T), 0, st, d, T, g, share);
+}
 template <int XT, int FT, int NV, bool WAVE>
 static void fwd_launch(const mscl_res_norm_desc& d, int T, unsigned grid, int64_t share, hipStream_t st) {
   const bool each = d.gate && d.rows_per_gate == 1, bias = d.b_post || d.b_pre;
-  const FastDiv g = make_fastdiv(d.gate ? (int)d.rows_per_gate : 1);
-  const dim3 th(WAVE ? 256 : T);
-  if (each) { if (bias) hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, true, true>), dim3(grid), th, 0, st, d, T, g, share);
-              else hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, true, false>), dim3(grid), th, 0, st, d, T, g, share); }
-  else { if (bias) hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, false, true>), dim3(grid), th, 0, st, d, T, g, share);
-         else hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, false, false>), dim3(grid), th, 0, st, d, T, g, share); }
+  if constexpr (NV == 1 && WAVE) {
+    if (d.C < 8) {
+      if (each) fwd_go<XT, FT, NV, WAVE, true, true, true>(d, T, grid, share, st);
+      else fwd_go<XT, FT, NV, WAVE, false, true, true>(d, T, grid, share, st);
+      return;
+    }
+  }
+  if (each) { if (bias) fwd_go<XT, FT, NV, WAVE, true, true>(d, T, grid, share, st); else fwd_go<XT, FT, NV, WAVE, true, false>(d, T, grid, share, st); }
+  else { if (bias) fwd_go<XT, FT, NV, WAVE, false, true>(d, T, grid, share, st); else fwd_go<XT, FT, NV, WAVE, false, false>(d, T, grid, share, st); }
 }
 template <int XT, int FT>
 void res_norm_fwd_types(const mscl_res_norm_desc& d, hipStream_t st) {
@@ -559,18 +618,26 @@ void res_norm_fwd_types(const mscl_res_norm_desc& d, hipStream_t st) {
   if (wave) { if (nv == 1) fwd_launch<XT, FT, 1, true>(d, T, (unsigned)grid, share, st); else fwd_launch<XT, FT, 2, true>(d, T, (unsigned)grid, share, st); }
   else { if (nv == 1) fwd_launch<XT, FT, 1, false>(d, T, (unsigned)grid, share, st); else fwd_launch<XT, FT, 2, false>(d, T, (unsigned)grid, share, st); }
 }
-template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS>
+template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS, bool NARROW = false>
 static void bwd_go(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
-  hipLaunchKernelGGL((res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS>), dim3(p.blocks), dim3(WAVE ? 256 : p.T), WAVE ? 256 * 8 * NV * 4 : 0, st, d, p);
+  hipLaunchKernelGGL((res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), dim3(p.blocks), dim3(WAVE ? 256 : p.T), WAVE ? 256 * 8 * NV * 4 : 0, st, d, p);
 }
 template <int XT, int FT, int NV, bool WAVE, int THREADS>
 static void bwd_launch(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
-  // the rare forms (rows past 8192 channels, short runs per gate) carry the bias sums always
+  // the rare forms (rows below 8 channels, short runs per gate) carry the bias sums always
+  if constexpr (WAVE) {
+    if (d.C < 8) {
+      if (p.mode == WHOLE) bwd_go<XT, FT, NV, WAVE, THREADS, WHOLE, true, true>(d, p, st);
+      else if (p.mode == SPLIT) bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, true, true>(d, p, st);
+      else bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, true, true>(d, p, st);
+      return;
+    }
+  }
   if (p.mode == WHOLE) return bwd_go<XT, FT, NV, WAVE, THREADS, WHOLE, true>(d, p, st);
-  if (NV > 1 || d.b_post || d.b_pre) {
+  if (d.b_post || d.b_pre) {
     if (p.mode == SPLIT) bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, true>(d, p, st);
     else bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, true>(d, p, st);
-  } else if constexpr (NV == 1) {
+  } else {
     if (p.mode == SPLIT) bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, false>(d, p, st);
     else bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, false>(d, p, st);
   }
@@ -580,6 +647,7 @@ int res_norm_bwd_types(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_
   if (p.wave) bwd_launch<XT, FT, 1, true, 256>(d, p, st);
   else if (p.nv == 2) bwd_launch<XT, FT, 2, false, 1024>(d, p, st);
   else if (p.T <= 512) bwd_launch<XT, FT, 1, false, 512>(d, p, st);
+  else if (p.T <= 768) bwd_launch<XT, FT, 1, false, 768>(d, p, st);        // 168 registers a lane; 1024 lanes leave 128
   else bwd_launch<XT, FT, 1, false, 1024>(d, p, st);
   MSCL_LAUNCH_CHECK();
   const int cols = d.C < 1024 ? 4 : 16;

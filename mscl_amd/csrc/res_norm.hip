@@ -27,16 +27,13 @@ static int res_norm_check(const mscl_res_norm_desc* d) {
 void res_norm_team(int C, int max_wave_nv, int* T, int* wave, int* nv) {
   *nv = 1;
   *wave = 1;
-  for (int t = 1; t <= 16; t *= 2) if (C <= 8 * t) { *T = t; return; }
-  if (C <= 256 && max_wave_nv == 2) { *T = 16; *nv = 2; return; }
-  if (C <= 512) { *T = 64; return; }
+  for (int t = 1; t <= 64; t *= 2) if (C <= 8 * t) { *T = t; return; }
   if (C <= 1024 && max_wave_nv == 2) { *T = 64; *nv = 2; return; }
   *wave = 0;
   *nv = C > 8192 ? 2 : 1;
   const int need = (C + 8 * *nv - 1) / (8 * *nv);
   *T = (need + 63) / 64 * 64;
 }
-
 extern "C" int mscl_res_norm_fwd(const mscl_res_norm_desc* d, void* stream) {
   const int rc = res_norm_check(d);
   if (rc) return rc;
