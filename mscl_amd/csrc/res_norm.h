@@ -277,7 +277,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void res_norm_fwd_kernel(mscl_re
       if (EACH_GATE) {
         act_row<false, NV>(d.gate_act, a, nullptr);
       } else if (d.gate) {
-        const int g = fdiv((int)r, gdiv);
+        const int g = d.rows_per_gate < d.rows ? fdiv((int)r, gdiv) : 0;
         if (g != gate) {
           gate = g;
           c.template load<FT>(d.gate, (int64_t)g * d.C, a);
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(512) void res_norm_finish_kernel(mscl_res_norm_desc
 void res_norm_team(int C, int max_wave_nv, int* T, int* wave, int* nv);
 template <int XT, int FT, int NV, bool WAVE, bool EACH, bool BIAS, bool NARROW = false>
 static void fwd_go(const mscl_res_norm_desc& d, int T, unsigned grid, int64_t share, hipStream_t st) {
-  const FastDiv g = make_fastdiv(d.gate ? (int)d.rows_per_gate : 1);
+  const FastDiv g = make_fastdiv(d.gate && d.rows_per_gate < d.rows ? (int)d.rows_per_gate : 1);        // below 2^30, as it has to be
   hipLaunchKernelGGL((res_norm_fwd_kernel<XT, FT, NV, WAVE, EACH, BIAS, NARROW>), dim3(grid), dim3(WAVE ? 256 : T), 0, st, d, T, g, share);
 }
 template <int XT, int FT, int NV, bool WAVE>

@@ -604,6 +604,9 @@ def _rows_of(t, C):
     return t.contiguous(), C
 
 
+_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device          # (a fifth of the host time; no lazy initialisation: tensors on the GPU are there)
+
+
 def _at(t):
     return None if t is None else t.data_ptr()
 
@@ -615,7 +618,7 @@ def _empty(t, dtype):
 
 class ResNormSaved:
     """what res_norm_bwd needs of a forward call"""
-    __slots__ = ('x', 'f', 'gate', 'vec', 'stats', 'codes', 'eps', 'shape', 'dims')
+    __slots__ = ('x', 'f', 'gate', 'vec', 'stats', 'desc', 'names', 'shape', 'kind')
 
 
 def _res_norm_check(x, f, gate, vec, post_norm, pre_norm, gate_act, eps):
@@ -669,7 +672,7 @@ def res_norm_fwd(x, f=None, *, gate=None, gate_act='sigmoid', scale=None, post_n
     rows, C, per = _res_norm_check(x, f, gate, vec, post_norm, pre_norm, gate_act, eps)
     if not x.is_cuda:
         raise lib.MsclError('mscl_amd kernels run on the GPU only (got a CPU tensor); there is no CPU fallback')
-    if torch.cuda.current_device() != x.device.index:
+    if _current_device() != x.get_device():
         with torch.cuda.device(x.device):
             return res_norm_fwd(x, f, gate=gate, gate_act=gate_act, post_norm=post_norm, pre_norm=pre_norm, eps=eps, save=save, **vec)
     x, ld_x = _rows_of(x, C)
@@ -687,17 +690,18 @@ def res_norm_fwd(x, f=None, *, gate=None, gate_act='sigmoid', scale=None, post_n
         want = (post_norm == 'layer', post_norm is not None, pre_norm == 'layer', pre_norm is not None)
         held = iter(torch.empty((sum(want), rows), dtype=torch.float32, device=x.device).unbind(0))
         stats = [next(held) if w else None for w in want]
+    d = lib.ResNormDesc(x.data_ptr(), _at(f), _at(gate), _at(scale), _at(w_post), _at(b_post), _at(w_pre), _at(b_pre),
+                        y.data_ptr() if f is not None else None, _at(h), _at(stats[0]), _at(stats[1]), _at(stats[2]), _at(stats[3]))
+    d.rows, d.ld_x, d.ld_f, d.rows_per_gate, d.C, d.x_type, d.f_type = rows, ld_x, ld_f, per, C, _TYPE_CODE[x.dtype], _TYPE_CODE[kind]
+    d.post, d.pre, d.gate_act, d.eps = NORMS[post_norm], NORMS[pre_norm], GATES[gate_act], eps
     if rows:
-        d = lib.ResNormDesc(x.data_ptr(), _at(f), _at(gate), _at(scale), _at(w_post), _at(b_post), _at(w_pre), _at(b_pre),
-                            y.data_ptr() if f is not None else None, _at(h), *[_at(t) for t in stats])
-        d.rows, d.ld_x, d.ld_f, d.rows_per_gate, d.C, d.x_type, d.f_type = rows, ld_x, ld_f, per, C, _TYPE_CODE[x.dtype], _TYPE_CODE[kind]
-        d.post, d.pre, d.gate_act, d.eps = NORMS[post_norm], NORMS[pre_norm], GATES[gate_act], eps
         call('mscl_res_norm_fwd', ctypes.byref(d), stream_ptr())
     if not save:
         return y, h, None
     saved = ResNormSaved()
-    saved.x, saved.f, saved.gate, saved.vec, saved.stats, saved.eps, saved.shape = x, f, gate, vec, stats, eps, tuple(x.shape)
-    saved.codes, saved.dims = (NORMS[post_norm], NORMS[pre_norm], GATES[gate_act]), (rows, C, per, ld_x, ld_f)
+    saved.x, saved.f, saved.gate, saved.vec, saved.stats, saved.desc = x, f, gate, vec, stats, d
+    saved.shape, saved.kind = x.shape, kind
+    saved.names = [k for k, t in (('x', x), ('f', f), ('gate', gate)) if t is not None] + [k for k in _VECTORS if vec[k] is not None]
     return y, h, saved
 
 
@@ -705,48 +709,44 @@ def res_norm_bwd(saved, dy=None, dh=None, into=None, need=None):
     """Gradients of res_norm_fwd from dy (of y, or of x itself where there was no f) and / or dh.  Returns a dict with 'x', 'f', 'gate',
     'scale', 'w_post', 'b_post', 'w_pre', 'b_pre' for what the forward was given (per-channel ones in fp32).  into: {name: fp32 vector} to
     ADD those per-channel gradients to instead -- all of them or none.  need: names to compute (None: all)."""
-    x, f, gate, vec = saved.x, saved.f, saved.gate, saved.vec
-    rows, C, per, ld_x, ld_f = saved.dims
-    post, pre, act = saved.codes
-    kind = x.dtype if f is None else f.dtype
+    x, d = saved.x, saved.desc
+    C, rows, dev = d.C, d.rows, x.device
     if dy is None and dh is None:
         raise lib.MsclError('res_norm_bwd needs dy or dh')
-    if dh is not None and not pre:
+    if dh is not None and not d.pre:
         raise lib.MsclError('res_norm_bwd: dh without pre_norm')
-    for g, t, what in ((dy, x.dtype, 'dy'), (dh, kind, 'dh')):
-        if g is not None and (tuple(g.shape) != saved.shape or g.dtype != t or g.device != x.device):
+    for g, t, what in ((dy, x.dtype, 'dy'), (dh, saved.kind, 'dh')):
+        if g is not None and (g.shape != saved.shape or g.dtype is not t or g.device != dev):
             raise lib.MsclError(f'res_norm_bwd: {what} is {tuple(saved.shape)} {t}, got {tuple(g.shape)} {g.dtype}')
-    names = [k for k in ('x', 'f', 'gate') + _VECTORS if k == 'x' or (f if k == 'f' else gate if k == 'gate' else vec[k]) is not None]
-    names = [k for k in names if need is None or k in need]
+    names = saved.names if need is None else [k for k in saved.names if k in need]
     if into is not None:
         for k in names:
-            if k in _VECTORS and (k not in into or into[k].dtype != torch.float32 or into[k].numel() != C or not into[k].is_contiguous() or into[k].device != x.device):
+            if k in _VECTORS and (k not in into or into[k].dtype != torch.float32 or into[k].numel() != C or not into[k].is_contiguous() or into[k].device != dev):
                 raise lib.MsclError(f'res_norm_bwd: into[{k!r}] is a contiguous fp32 vector of {C} channels beside x')
-    if torch.cuda.current_device() != x.device.index:
-        with torch.cuda.device(x.device):
+    if _current_device() != x.get_device():
+        with torch.cuda.device(dev):
             return res_norm_bwd(saved, dy, dh, into, need)
     dy = dy.contiguous() if dy is not None else None
     dh = dh.contiguous() if dh is not None else None
     out = {}
-    made = [k for k in names if k in _VECTORS] if into is None else ()
-    if made:                                             # one allocation; zeros where nothing reaches them
+    made = [k for k in names if k in _VECTORS]
+    if into is not None:
+        out = {k: into[k] for k in made}
+    elif made:                                           # one allocation; zeros where nothing reaches them
         unreached = rows == 0 or (dh is None and any(k.endswith('pre') for k in made))
-        out = dict(zip(made, (torch.zeros if unreached else torch.empty)((len(made), C), dtype=torch.float32, device=x.device).unbind(0)))
+        out = dict(zip(made, (torch.zeros if unreached else torch.empty)((len(made), C), dtype=torch.float32, device=dev).unbind(0)))
     for k in names:
-        if k in _VECTORS:
-            if into is not None:
-                out[k] = into[k]
-        else:
-            src = x if k == 'x' else f if k == 'f' else gate
+        if k not in out:
+            src = getattr(saved, k)
             out[k] = _empty(src, src.dtype)
     if rows == 0:
         return out
-    d = lib.ResNormDesc(x.data_ptr(), _at(f), _at(gate), *[_at(vec[k]) for k in _VECTORS], None, None, *[_at(t) for t in saved.stats], _at(dy), _at(dh),
-                        *[_at(out.get(k)) for k in ('x', 'f', 'gate') + _VECTORS])
-    d.rows, d.ld_x, d.ld_f, d.rows_per_gate, d.C, d.x_type, d.f_type = rows, ld_x, ld_f, per, C, _TYPE_CODE[x.dtype], _TYPE_CODE[kind]
-    d.post, d.pre, d.gate_act, d.accumulate, d.eps = post, pre, act, int(into is not None), saved.eps
+    d = lib.ResNormDesc.from_buffer_copy(d)
+    d.dy, d.dh, d.accumulate = _at(dy), _at(dh), int(into is not None)
+    for k, v in out.items():
+        setattr(d, 'd' + k, v.data_ptr())
     n = lib.call_raw('mscl_res_norm_ws', ctypes.byref(d))
-    ws = torch.empty(n, dtype=torch.float32, device=x.device)
+    ws = torch.empty(n, dtype=torch.float32, device=dev)
     d.ws, d.ws_floats = ws.data_ptr(), n
     call('mscl_res_norm_bwd', ctypes.byref(d), stream_ptr())
     return out

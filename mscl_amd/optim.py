@@ -184,8 +184,8 @@ def _check_grad_memory(ptrs, nbytes, spans):
 def _check_args(lr, betas, eps, weight_decay, grad_clip, state_bits, seed=0):
     if state_bits not in (32, 8):
         raise MsclError(f'AdamW: state_bits is 32 or 8, not {state_bits}')
-    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps > 0 and lr >= 0 and weight_decay >= 0):
-        raise MsclError('AdamW: needs 0 <= betas < 1, eps > 0, lr >= 0, weight_decay >= 0')
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and np.float32(eps) > 0 and lr >= 0 and weight_decay >= 0):
+        raise MsclError('AdamW: needs 0 <= betas < 1, eps > 0 in fp32, lr >= 0, weight_decay >= 0')
     if grad_clip is not None and grad_clip.get('norm_type', 2) != 2:
         raise NotImplementedError('only the L2 norm is used (optimizer_config.grad_clip.norm_type=2)')
     if grad_clip is not None and not grad_clip['max_norm'] > 0:
@@ -223,6 +223,7 @@ class AdamW:
         if not self.params[0].is_cuda:
             raise MsclError('mscl_amd kernels run on the GPU only (got a CPU tensor); there is no CPU fallback')
         self._param_ptrs = [p.data_ptr() for p in self.params]
+        self._shapes, self._strides = [p.shape for p in self.params], [p.stride() for p in self.params]
         self.betas, self.eps, self.wd, self.state_bits, self.seed = (float(betas[0]), float(betas[1])), float(eps), float(weight_decay), state_bits, int(seed)
         self.max_norm = float(grad_clip['max_norm']) if grad_clip else 0.0
         self.param_groups = [dict(lr=lr, betas=self.betas, eps=self.eps, weight_decay=self.wd)]
@@ -271,11 +272,18 @@ class AdamW:
         return self._norm[0]
 
     def _set_grads(self, grads):
-        if [p.data_ptr() for p in self._leaves] != self._param_ptrs:
+        T = torch.Tensor
+        if list(map(T.data_ptr, self._leaves)) != self._param_ptrs:
             raise MsclError('AdamW: a parameter has moved to other memory since the optimizer was built')
         grads = [p.grad for p in self._leaves] if grads is None else list(grads)
-        _check_grads(grads, self.params)
-        ptrs = [g.data_ptr() for g in grads]
+        try:            # all at once for many tensors (hundreds of them cost more host time than a small step takes)
+            alike = ([g.shape for g in grads] == self._shapes and list(map(T.stride, grads)) == self._strides and
+                     len({g.dtype for g in grads}) == 1 and grads[0].dtype in _TYPES and set(map(T.get_device, grads)) == {self.device.index})
+        except (AttributeError, TypeError):
+            alike = False
+        if not alike:   # one by one: names what does not fit, or finds that it does
+            _check_grads(grads, self.params)
+        ptrs = list(map(T.data_ptr, grads))
         if ptrs != self._grad_ptrs:
             _check_grad_memory(ptrs, [g.numel() * g.element_size() for g in grads], self._spans)
             if self._in_graph:                  # a captured step reads the old table: leave it as it is, with its gradients' addresses

@@ -29,6 +29,7 @@ def test_refusals_on_the_host():
     bad('betas', [a], betas=(1.0, 0.9))
     bad('betas', [a], betas=(0.9, float('nan')))
     bad('eps', [a], eps=0.0)
+    bad('eps', [a], eps=1e-60)
     bad('weight_decay', [a], weight_decay=-1.0)
     bad('L2', [a], grad_clip=dict(max_norm=1.0, norm_type=1))
     bad('max_norm', [a], grad_clip=dict(max_norm=0.0))
@@ -390,3 +391,36 @@ def test_other_stream_state_dict_and_layouts(dev):
         o.step([torch.zeros(10, device=dev)])
     with pytest.raises(MsclError, match='share memory'):
         AdamW([twin], lr=1e-3).step([twin])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+def test_offsets_past_32_bits(bits, dev):
+    """one tensor of 2^32 + 1000 elements (34 to 60 GB): its last elements against the formula, and a tensor behind it"""
+    from mscl_amd import AdamW
+    n, tail = (1 << 32) + 1000, 3000
+    p, g = torch.zeros(n, device=dev), torch.zeros(n, dtype=torch.bfloat16, device=dev)
+    gen = torch.Generator().manual_seed(2)
+    p[-tail:].copy_(torch.randn(tail, generator=gen))
+    g[-tail:].copy_(torch.randn(tail, generator=gen) * 0.01)
+    p2, g2 = torch.ones(77, device=dev), torch.full((77,), 0.01, dtype=torch.bfloat16, device=dev)
+    P, G = p[-tail:].cpu().double().numpy(), g[-tail:].cpu().double().numpy()
+    opt = AdamW([p, p2], lr=1e-2, weight_decay=0.1, grad_clip=dict(max_norm=0.05), state_bits=bits, seed=5)
+    opt.step([g, g2])
+    coef, norm = oracle.coefficient([G, g2.cpu().double().numpy()], 0.05)
+    assert coef < 1 and abs(float(opt.grad_norm()) - norm) <= 2 * U * norm
+    lr = float(np.float32(1e-2))
+    _, m, v = oracle.step(P, G, np.zeros(tail), np.zeros(tail), 1, coef, lr)
+    _check_p(p[-tail:].cpu().double().numpy(), P, m, v, np.abs(m), 1, lr, 0.1, (0.9, 0.999), 1e-8, 'tail')
+    assert not p[:n - tail].any()
+    if bits == 32:
+        assert (np.abs(opt.exp_avg[n - tail:n].cpu().double().numpy() - m) <= 6 * U * np.abs(m)).all()
+    else:                                   # whole blocks only: from the first block boundary inside the tail
+        o = -(-(n - tail) // 256) * 256
+        k = o - (n - tail)
+        lo, hi = oracle.random_bits(n - o, o, 5, 1)
+        for got, want, r, b in ((opt.exp_avg, m[k:], lo, 4), (opt.exp_avg_sq, v[k:], hi, 5)):
+            e = opt.exponents[b - 4, o // 256:-(-n // 256)].cpu().numpy()
+            q, _, _ = oracle.quantise(want, r, b)
+            assert (oracle.decode(got[o:n].cpu().numpy(), e, b) != q).sum() <= 2
+    assert opt.offsets == [0, -(-n // 256) * 256] and bool((p2 < 1).all())

@@ -300,13 +300,30 @@ def test_offsets_past_32_bits(dev):
     rows, C = (1 << 25) + 17, 64
     f = torch.empty(rows, C, dtype=BF, device=dev)
     f.normal_()
-    x = f.flip(0) if False else f
+    x = f
     y, h, s = K_.res_norm_fwd(x, f, post_norm='rms', pre_norm='layer', save=True)
     y2, h2, s2 = K_.res_norm_fwd(x[-40:], f[-40:], post_norm='rms', pre_norm='layer', save=True)
     assert torch.equal(y[-40:], y2) and torch.equal(h[-40:], h2)
     g = K_.res_norm_bwd(s, f, f, need=('x', 'f'))
     g2 = K_.res_norm_bwd(s2, f[-40:], f[-40:], need=('x', 'f'))
     assert torch.equal(g['x'][-40:], g2['x']) and torch.equal(g['f'][-40:], g2['f'])
+
+
+@pytest.mark.gpu
+def test_one_gate_for_over_a_billion_rows(dev):
+    from mscl_amd import kernels as K_
+    rows = (1 << 30) + 40
+    x = torch.ones(rows, 1, dtype=BF, device=dev)
+    gate = torch.full((1, 1), 0.5, dtype=BF, device=dev)
+    x[-40:] = torch.arange(40, dtype=BF, device=dev)[:, None]
+    y, _, s = K_.res_norm_fwd(x, x, gate=gate, save=True)
+    a = torch.sigmoid(torch.tensor(0.5))
+    want = (x[-45:].float() * (1 + float(a))).bfloat16()
+    assert float((y[-45:].float() - want.float()).abs().max()) <= 2.0 ** -7 * 64          # one step of the largest value, 39 a
+    g = K_.res_norm_bwd(s, x)
+    assert float((g['x'][-45:].float() - x[-45:].float()).abs().max()) == 0
+    total = float(a * (1 - a)) * (float(rows - 40) + sum(i * i for i in range(40)))
+    assert abs(float(g['gate']) / total - 1) <= 2.0 ** -8 + 1e-3                          # bf16, and fp32 sums over 2^30 ones
 
 
 @pytest.mark.gpu
