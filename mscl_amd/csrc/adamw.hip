@@ -12,17 +12,23 @@
 // pattern: after ldexp has put the code's smallest normal exponent onto fp32's own, code = (bits + random) >> 20, subnormals included.
 // The rounding is stochastic because b2 = 0.999 moves v by 0.1 % a step and 3 mantissa bits are 6-12 %: a nearest rounding would never move
 // it.  p is updated from the moments BEFORE they are rounded.
+//
+// What bounds it (MI355X, where a copy of 4 GB runs at 4.8 TB/s and an in-place add at 5.9): memory.  Counters give the bytes of the
+// formula and no more: 26 per element for 16-bit gradients and no shadow, 320 M elements in 1.48 ms = 5.6 TB/s; 33 M elements with fp32
+// gradients, a clip and a shadow (30 bytes, 4 more where the gradient is read a second time, partly from the last-level cache): 26 us for the
+// norm, 5 for the coefficient, 153 for the update.  8 bits: 16 bytes per element, 300 M in 0.85 ms = 5.7 TB/s with the vector units busy
+// about four fifths of the time (78 instructions per element, two of them quarter-rate multiplies of the hash).
 #include "common.h"
 #include <hip/hip_fp16.h>
 
 namespace {
-constexpr int CHUNK = 4096;          // elements a block of 256 threads takes: 4 vectors of 4 per thread and array
+constexpr int CHUNK = 4096;          // elements a block of 256 threads takes: 4 vectors of 4 per thread and array, 16 loads in flight (32 bits)
 constexpr int PARTS = MSCL_ADAMW_PARTS;
 
 struct Words { int64_t step; float c1, c2; uint32_t key, seed; float coef; uint32_t pad; };      // = the words buffer
 
 // The update passes once over far more memory than any cache holds: its accesses are marked non-temporal, which leaves the caches to the
-// gradient between the two launches (33 M elements, fp32 / clip / shadow: 238 -> 200 us; 320 M without clip: 1611 -> 1507 us).
+// gradient between the launches (33 M elements, fp32 / clip / shadow: a step of 238 -> 200 us; 320 M without clip: 1611 -> 1507 us).
 __device__ __forceinline__ float4 ldnt(const float* p) {
   const f32x4_t v = __builtin_nontemporal_load((const f32x4_t*)p);
   return make_float4(v[0], v[1], v[2], v[3]);
@@ -224,7 +230,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(mscl_adamw_desc d, int parts
     }
   }
   float coef = w->coef;
-  if (parts) {                                                   // few partials: every block adds them up, in the same order
+  if (parts) {                                                   // not added up yet: every block does, in the same order
     add_partials(d, parts, red);
     coef = clip_coef(d, red, blockIdx.x == 0 && tid == 0);
   }
@@ -313,10 +319,11 @@ static int adamw_launch(const mscl_adamw_desc& d, hipStream_t st) {
   if (d.max_norm > 0.0) blocks = d.n_chunks < PARTS ? d.n_chunks : PARTS;
   hipLaunchKernelGGL(adamw_prelude_kernel<GT>, dim3((unsigned)blocks), dim3(256), 0, st, d);
   MSCL_LAUNCH_CHECK();
-  // Up to 256 partials (a million elements) the update's blocks add them up themselves; more are added once, in a launch of their own.
-  // (The last block of launch 1 adding them -- a ticket and a release per block -- took 90 us for 2048 blocks.)
+  // Up to 16 M elements the update's blocks add the partials up themselves, each all of them; from there on they are added once, in a launch of
+  // its own: a step of 4 / 8 / 16 / 33 / 100 M elements 25 / 49 / 94 / 193 / 573 us without it, 30 / 53 / 93 / 179 / 546 us with it.  (The last
+  // block of launch 1 adding them -- a ticket and a release per block -- took 90 us for 2048 blocks.)
   int parts = d.max_norm > 0.0 ? (int)blocks : 0;
-  if (parts > 256) {
+  if (parts && d.n_chunks > 4096) {
     hipLaunchKernelGGL(adamw_coef_kernel, dim3(1), dim3(256), 0, st, d, parts);
     MSCL_LAUNCH_CHECK();
     parts = 0;

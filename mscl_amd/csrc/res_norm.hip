@@ -23,12 +23,12 @@ static int res_norm_check(const mscl_res_norm_desc* d) {
   if (d->gate && (!d->f || d->rows_per_gate <= 0 || d->rows % d->rows_per_gate)) return MSCL_E_SHAPE;
   return 0;
 }
-// lanes of a row: the fewest that hold it at 8 NV channels each
-void res_norm_team(int C, int max_wave_nv, int* T, int* wave, int* nv) {
+// Lanes of a row: the fewest that hold it at 8 NV channels each -- a power of two up to 64, then whole waves.  (16 channels a lane in one wave
+// for 513 .. 1024 channels: forward of 24 M elements bf16 / fp32 35.3 / 52.2 us at 1024, 33.9 / 49.6 us with two waves.)
+void res_norm_team(int C, int* T, int* wave, int* nv) {
   *nv = 1;
   *wave = 1;
   for (int t = 1; t <= 64; t *= 2) if (C <= 8 * t) { *T = t; return; }
-  if (C <= 1024 && max_wave_nv == 2) { *T = 64; *nv = 2; return; }
   *wave = 0;
   *nv = C > 8192 ? 2 : 1;
   const int need = (C + 8 * *nv - 1) / (8 * *nv);
@@ -50,13 +50,18 @@ extern "C" int mscl_res_norm_fwd(const mscl_res_norm_desc* d, void* stream) {
 
 static BwdPlan bwd_plan(const mscl_res_norm_desc* d) {
   BwdPlan p;
-  res_norm_team(d->C, 1, &p.T, &p.wave, &p.nv);
+  res_norm_team(d->C, &p.T, &p.wave, &p.nv);
   const int per = p.wave ? 256 / p.T : 1;
   // blocks for 256 CUs of 16 waves (128 registers a lane); every block costs up to 4 C floats of column sums
   const int target = p.wave ? 1024 : 4096 / (p.T / 64);
   p.rows_per_gate = (int)(d->gate ? d->rows_per_gate : d->rows);
   p.gates = (int)(d->rows / p.rows_per_gate);
-  p.mode = !d->gate ? SPLIT : p.rows_per_gate == 1 ? EACH1 : p.rows_per_gate < 16 || p.gates >= 4 * target * per ? WHOLE : SPLIT;
+  // Many short runs: a team each.  (24 M elements, bf16, C = 64 / 512 / 2048, a training pass, WHOLE against SPLIT: runs of 4 rows 129 / 128 /
+  // 124 against 1335 / 270 / 207 us, 16 rows 113 / 110 / 112 against 384 / 138 / 134, 32 rows 128 / 119 / 124 against 235 / 125 / 129, 64 rows
+  // 153 / 148 / 161 against 163 / 121 / 128.)  Few runs of any length leave most teams without one.
+  const int teams = target * per;
+  const bool many = p.gates >= 4 * teams || (p.rows_per_gate <= 32 && p.gates >= (teams / 2 < 1024 ? teams / 2 : 1024));
+  p.mode = !d->gate ? SPLIT : p.rows_per_gate == 1 ? EACH1 : many ? WHOLE : SPLIT;
   if (p.mode != SPLIT) {
     p.per_gate = 1;
     const int64_t need = cdiv64(p.gates, per);
