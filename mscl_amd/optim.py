@@ -285,6 +285,8 @@ class AdamW:
             _check_grads(grads, self.params)
         ptrs = list(map(T.data_ptr, grads))
         if ptrs != self._grad_ptrs:
+            if torch.cuda.is_current_stream_capturing():
+                raise MsclError('AdamW: a step is captured with the gradient tensors of the eager step before it (a capture cannot upload other addresses)')
             _check_grad_memory(ptrs, [g.numel() * g.element_size() for g in grads], self._spans)
             if self._in_graph:                  # a captured step reads the old table: leave it as it is, with its gradients' addresses
                 self._kept.append(self._grad_ring)
@@ -302,18 +304,22 @@ class AdamW:
         self._launch()
 
     def _launch(self):
-        if torch.cuda.is_current_stream_capturing():        # a captured step publishes before each replay
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
             self._in_graph = True
-        else:
+        else:                                               # a captured step publishes before each replay
             self.sync_lr()
-            self.steps += 1
         lib.call('mscl_adamw_step', ctypes.byref(self._desc), lib.stream_ptr())
+        self.steps += not capturing
 
     def sync_lr(self):
         """publish param_groups[0]['lr'] to the device word the kernel reads, in stream order.  Unchanged values are not re-sent."""
         lr = float(self.param_groups[0]['lr'])
         if lr == self._lr_sent:
             return
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.sync_lr()
         self._lr_cpu[0] = lr
         self._lr.push(self._lr_cpu)
         self._lr_sent = lr
@@ -446,6 +452,8 @@ class ClipAdamW:
         else:
             parallel.allreduce_mean_(ar.G)
         if self._inner is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise MsclError('ClipAdamW: take one eager step before capturing one')
             self._build()
         elif [s for s in ar.slots if s.touched] != self._slots:
             raise RuntimeError('the set of parameters receiving gradients changed between steps')

@@ -348,11 +348,29 @@ def test_captured_step_replays(bits, dev):
     assert int(runs[0][-1]) == 6
     for a, b in zip(*runs):
         assert torch.equal(a, b)
+    from mscl_amd.lib import MsclError
     ps, gs, _ = _make(sizes, dev, 6)
     opt = AdamW(ps)
-    with pytest.raises(RuntimeError, match='capture'):
+    with pytest.raises(MsclError, match='capture'):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             opt.step(gs)                      # no eager step before: the addresses cannot be uploaded inside a capture
+    # the same after a captured step; the refused one leaves eager and captured steps as they were
+    twin = AdamW([p.clone() for p in ps], state_bits=bits)
+    opt = AdamW(ps, state_bits=bits)
+    opt.step(gs)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step(gs)
+    others = [g.clone() for g in gs]
+    with pytest.raises(MsclError, match='capture'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step(others)
+    opt.step(gs)
+    graph.replay()
+    for _ in range(3):
+        twin.step(gs)
+    assert opt.device_step() == 3 and all(torch.equal(a, b) for a, b in zip(ps, twin.params))
 
 
 @pytest.mark.gpu
