@@ -41,6 +41,8 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
 __device__ __forceinline__ uint2 ldnt(const uint2* p) { const u32x2_t v = __builtin_nontemporal_load((const u32x2_t*)p); return make_uint2(v[0], v[1]); }
 __device__ __forceinline__ void stnt(uint2* p, uint2 v) { const u32x2_t u = {v.x, v.y}; __builtin_nontemporal_store(u, (u32x2_t*)p); }
 __device__ __forceinline__ float4 ldnt(const float4* p) { return ldnt((const float*)p); }
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+__device__ __forceinline__ void stnt(uint4* p, uint4 v) { const u32x4_t u = {v.x, v.y, v.z, v.w}; __builtin_nontemporal_store(u, (u32x4_t*)p); }
 
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {          // finaliser of MurmurHash3 (Appleby, public domain)
   x ^= x >> 16; x *= 0x85EBCA6Bu; x ^= x >> 13; x *= 0xC2B2AE35u; x ^= x >> 16;
@@ -351,12 +353,13 @@ extern "C" int mscl_adamw_step(const mscl_adamw_desc* d, void* stream) {
   return MSCL_E_SHAPE;
 }
 
-// The values that 8-bit states stand for, as bf16 (exact: 4 significant bits, bf16 has 8).  A thread decodes 8 elements.
+// The values that 8-bit states stand for, as bf16 (exact: 4 significant bits, bf16 has 8).  A thread decodes 8 elements.  Bound by memory:
+// 300 M elements, 1.8 GB, 345 us.  Non-temporal like the update (a step and its values at 32 / 300 M elements: 161 / 1169 us without, 154 / 1173 with).
 __global__ __launch_bounds__(256) void adamw_values_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v,
                                                            const uint8_t* __restrict__ ex, bf16_t* __restrict__ om, bf16_t* __restrict__ ov,
                                                            int64_t n_blocks) {
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n_blocks * 32; q += (int64_t)gridDim.x * 256) {
-    const uint2 a = ((const uint2*)m)[q], b = ((const uint2*)v)[q];
+    const uint2 a = ldnt((const uint2*)m + q), b = ldnt((const uint2*)v + q);
     const int Em = ex[q >> 5], Ev = ex[n_blocks + (q >> 5)];
     float fm[8], fv[8];
 #pragma unroll
@@ -365,8 +368,8 @@ __global__ __launch_bounds__(256) void adamw_values_kernel(const uint8_t* __rest
       fm[i] = Em == 255 ? __builtin_nanf("") : decode_m(ca, Em);
       fv[i] = Ev == 255 ? __builtin_nanf("") : decode_v(cb, Ev);
     }
-    ((uint4*)om)[q] = pack8(fm);
-    ((uint4*)ov)[q] = pack8(fv);
+    stnt((uint4*)om + q, pack8(fm));
+    stnt((uint4*)ov + q, pack8(fv));
   }
 }
 extern "C" int mscl_adamw_values(const uint8_t* m, const uint8_t* v, const uint8_t* exponents, uint16_t* m_out, uint16_t* v_out,
