@@ -15,8 +15,8 @@
 //
 // What bounds it (MI355X, where a copy of 4 GB runs at 4.8 TB/s and an in-place add at 5.9): memory.  Counters give the bytes of the
 // formula and no more: 26 per element for 16-bit gradients and no shadow, 320 M elements in 1.48 ms = 5.6 TB/s; 33 M elements with fp32
-// gradients, a clip and a shadow (30 bytes, 4 more where the gradient is read a second time, partly from the last-level cache): 26 us for the
-// norm, 5 for the coefficient, 153 for the update.  8 bits: 16 bytes per element, 300 M in 0.85 ms = 5.7 TB/s with the vector units busy
+// gradients, a clip and a shadow (30 bytes, 4 more where the gradient is read a second time, partly from the last-level cache): 25 us for the
+// norm, 5 for the coefficient, 151 for the update.  8 bits: 16 bytes per element, 300 M in 0.85 ms = 5.7 TB/s with the vector units busy
 // about four fifths of the time (78 instructions per element, two of them quarter-rate multiplies of the hash).
 #include "common.h"
 #include <hip/hip_fp16.h>
@@ -29,19 +29,23 @@ struct Words { int64_t step; float c1, c2; uint32_t key, seed; float coef; uint3
 
 // The update passes once over far more memory than any cache holds: its accesses are marked non-temporal, which leaves the caches to the
 // gradient between the launches (33 M elements, fp32 / clip / shadow: a step of 238 -> 200 us; 320 M without clip: 1611 -> 1507 us).
+// Vectors of 4 elements are accessed at the alignment of one (the memory path of gfx950 takes any): a view that starts anywhere takes the same
+// code, and of a tensor's last chunk only the vector that its end cuts goes element by element (161 tensors, 31.6 M elements: norm 34 -> 24 us).
+typedef f32x4_t f32x4_at4 __attribute__((aligned(4)));
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+typedef u32x2_t u32x2_at2 __attribute__((aligned(2)));
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 __device__ __forceinline__ float4 ldnt(const float* p) {
-  const f32x4_t v = __builtin_nontemporal_load((const f32x4_t*)p);
+  const f32x4_t v = __builtin_nontemporal_load((const f32x4_at4*)p);
   return make_float4(v[0], v[1], v[2], v[3]);
 }
 __device__ __forceinline__ void stnt(float* p, const float* v) {
   const f32x4_t u = {v[0], v[1], v[2], v[3]};
-  __builtin_nontemporal_store(u, (f32x4_t*)p);
+  __builtin_nontemporal_store(u, (f32x4_at4*)p);
 }
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+__device__ __forceinline__ uint2 ldnt(const uint16_t* p) { const u32x2_t v = __builtin_nontemporal_load((const u32x2_at2*)p); return make_uint2(v[0], v[1]); }
+__device__ __forceinline__ void stnt(uint16_t* p, uint2 v) { const u32x2_t u = {v.x, v.y}; __builtin_nontemporal_store(u, (u32x2_at2*)p); }
 __device__ __forceinline__ uint2 ldnt(const uint2* p) { const u32x2_t v = __builtin_nontemporal_load((const u32x2_t*)p); return make_uint2(v[0], v[1]); }
-__device__ __forceinline__ void stnt(uint2* p, uint2 v) { const u32x2_t u = {v.x, v.y}; __builtin_nontemporal_store(u, (u32x2_t*)p); }
-__device__ __forceinline__ float4 ldnt(const float4* p) { return ldnt((const float*)p); }
-typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 __device__ __forceinline__ void stnt(uint4* p, uint4 v) { const u32x4_t u = {v.x, v.y, v.z, v.w}; __builtin_nontemporal_store(u, (u32x4_t*)p); }
 
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {          // finaliser of MurmurHash3 (Appleby, public domain)
@@ -71,15 +75,24 @@ template <int GT> __device__ __forceinline__ float grad1(const void* g, int64_t 
   const uint16_t h = ((const uint16_t*)g)[e];
   return GT == MSCL_BF16 ? bf2f(h) : half2f(h);
 }
-template <int GT> struct GradVec { typedef uint2 type; };
-template <> struct GradVec<MSCL_F32> { typedef float4 type; };
-template <int GT> __device__ __forceinline__ float4 grad4(const typename GradVec<GT>::type& v);
-template <> __device__ __forceinline__ float4 grad4<MSCL_F32>(const float4& v) { return v; }
-template <> __device__ __forceinline__ float4 grad4<MSCL_BF16>(const uint2& v) {
-  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
-}
-template <> __device__ __forceinline__ float4 grad4<MSCL_F16>(const uint2& v) {
+// 4 gradients from element e on; NT: for the last time
+template <int GT, bool NT> __device__ __forceinline__ float4 grad4(const void* g, int64_t e) {
+  if (GT == MSCL_F32) {
+    if (NT) return ldnt((const float*)g + e);
+    const f32x4_t v = *(const f32x4_at4*)((const float*)g + e);
+    return make_float4(v[0], v[1], v[2], v[3]);
+  }
+  uint2 v;
+  if (NT) v = ldnt((const uint16_t*)g + e);
+  else { const u32x2_t u = *(const u32x2_at2*)((const uint16_t*)g + e); v = make_uint2(u[0], u[1]); }
+  if (GT == MSCL_BF16)
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
   return make_float4(half2f((uint16_t)v.x), half2f((uint16_t)(v.x >> 16)), half2f((uint16_t)v.y), half2f((uint16_t)(v.y >> 16)));
+}
+// the same where the tensor ends at element n: zeros from there on
+template <int GT, bool NT> __device__ __forceinline__ float4 grad4_end(const void* g, int64_t e, int64_t n) {
+  if (e + 4 <= n) return grad4<GT, NT>(g, e);
+  return make_float4(e < n ? grad1<GT>(g, e) : 0.f, e + 1 < n ? grad1<GT>(g, e + 1) : 0.f, e + 2 < n ? grad1<GT>(g, e + 2) : 0.f, 0.f);
 }
 __device__ __forceinline__ uint16_t f2half(float f) { return __half_as_ushort(__float2half_rn(f)); }
 template <int ST> __device__ __forceinline__ uint16_t shadow1(float f) { return ST == MSCL_BF16 ? f2bf(f) : f2half(f); }
@@ -132,33 +145,28 @@ __global__ __launch_bounds__(256) void adamw_prelude_kernel(mscl_adamw_desc d) {
     if (d.max_norm <= 0.0) w->coef = 1.f;
   }
   if (d.max_norm <= 0.0) return;
-  typedef typename GradVec<GT>::type vec_t;
-  constexpr uintptr_t mask = GT == MSCL_F32 ? 15 : 7;
-  constexpr int size = GT == MSCL_F32 ? 4 : 2;
   double s = 0.0;
   int chunk = blockIdx.x;                                    // the grid is no larger than the number of chunks
   int ti = d.chunk_tensor[chunk];
   int64_t n = d.tensors[ti].n, base = (int64_t)(chunk - d.tensors[ti].first_chunk) * CHUNK;
-  const char* g = (const char*)d.grads[ti];
+  const void* g = d.grads[ti];
   while (true) {
     const int64_t next = (int64_t)chunk + gridDim.x;
-    const bool more = next < d.n_chunks, whole = base + CHUNK <= n && ((uintptr_t)g & mask) == 0;
-    vec_t v[4];
-    if (whole)
+    const bool more = next < d.n_chunks;
+    float4 v[4];
+    if (base + CHUNK <= n) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = *(const vec_t*)(g + (base + k * 1024 + tid * 4) * size);
+      for (int k = 0; k < 4; ++k) v[k] = grad4<GT, false>(g, base + k * 1024 + tid * 4);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = grad4_end<GT, false>(g, base + k * 1024 + tid * 4, n);
+    }
     const int tn = more ? d.chunk_tensor[next] : ti;
     const int64_t n2 = d.tensors[tn].n, base2 = (next - d.tensors[tn].first_chunk) * CHUNK;
-    const char* g2 = (const char*)d.grads[tn];
-    if (whole) {
+    const void* g2 = d.grads[tn];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 f = grad4<GT>(v[k]);
-        s += (double)f.x * f.x; s += (double)f.y * f.y; s += (double)f.z * f.z; s += (double)f.w * f.w;
-      }
-    } else {
-      const int64_t end = base + CHUNK < n ? base + CHUNK : n;
-      for (int64_t e = base + tid; e < end; e += 256) { const double f = grad1<GT>(g, e); s += f * f; }
+    for (int k = 0; k < 4; ++k) {
+      s += (double)v[k].x * v[k].x; s += (double)v[k].y * v[k].y; s += (double)v[k].z * v[k].z; s += (double)v[k].w * v[k].w;
     }
     if (!more) break;
     chunk = (int)next; ti = tn; n = n2; base = base2; g = g2;
@@ -195,8 +203,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(mscl_adamw_desc d, int parts
   uint16_t* __restrict__ sh = T->shadow;
   const int64_t n = T->n, base = (int64_t)((int)blockIdx.x - T->first_chunk) * CHUNK, off = T->off + base;
   const Words* w = (const Words*)d.words;
-  constexpr uintptr_t gmask = GT == MSCL_F32 ? 15 : 7;
-  const bool vec = base + CHUNK <= n && ((uintptr_t)p & 15) == 0 && ((uintptr_t)g & gmask) == 0 && (ST == MSCL_NONE || ((uintptr_t)sh & 7) == 0);
+  const bool whole = base + CHUNK <= n;
 
   float pv[4][4], gv[4][4];
   float4 mv[4], vv[4];
@@ -207,16 +214,15 @@ __global__ __launch_bounds__(256) void adamw_kernel(mscl_adamw_desc d, int parts
   for (int k = 0; k < 4; ++k) {
     const int64_t e = base + k * 1024 + tid * 4;
     live[k] = base + k * 1024 + (tid & ~63) * 4 < n;            // wave-uniform: the 256 elements of this wave hold a live one
-    if (vec) {
+    if (whole) {
       *(float4*)pv[k] = ldnt(p + e);
-      *(float4*)gv[k] = grad4<GT>(ldnt((const typename GradVec<GT>::type*)((const char*)g + e * (GT == MSCL_F32 ? 4 : 2))));
+      *(float4*)gv[k] = grad4<GT, true>(g, e);
     } else {
+      if (e + 4 <= n) *(float4*)pv[k] = ldnt(p + e);
+      else
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = e + i < n;
-        pv[k][i] = in ? p[e + i] : 0.f;
-        gv[k][i] = in ? grad1<GT>(g, e + i) : 0.f;
-      }
+        for (int i = 0; i < 4; ++i) pv[k][i] = e + i < n ? p[e + i] : 0.f;
+      *(float4*)gv[k] = grad4_end<GT, true>(g, e, n);
     }
     if (live[k]) {                                               // the states are padded to whole 256-element blocks of zeros
       const int64_t s = off + k * 1024 + tid * 4;
@@ -264,13 +270,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(mscl_adamw_desc d, int parts
       const float den = __builtin_amdgcn_sqrtf(v[i]) * c2 + eps;
       pv[k][i] = pv[k][i] * keep - rate * m[i] * __builtin_amdgcn_rcpf(den);
     }
-    if (vec) {
+    if (whole || e + 4 <= n) {
       stnt(p + e, pv[k]);
       if (ST != MSCL_NONE) {
         uint2 b;
         b.x = shadow1<ST>(pv[k][0]) | (uint32_t)shadow1<ST>(pv[k][1]) << 16;
         b.y = shadow1<ST>(pv[k][2]) | (uint32_t)shadow1<ST>(pv[k][3]) << 16;
-        stnt((uint2*)(sh + e), b);
+        stnt(sh + e, b);
       }
     } else {
 #pragma unroll
