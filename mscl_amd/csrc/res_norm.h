@@ -319,7 +319,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void res_norm_fwd_kernel(mscl_re
 //   WHOLE  the gates are short or very many: a team takes whole gates, applies a itself and writes dgate at the end of each
 //   EACH1  a gate for every row: as WHOLE with runs of one row, and nothing to keep between rows but the totals
 enum { SPLIT = 0, WHOLE = 1, EACH1 = 2 };
-struct BwdPlan { int T, wave, nv, mode, per_gate, gates, blocks, rows_per_gate; };
+struct BwdPlan { int T, wave, nv, mode, per_gate, gates, blocks, rows_per_gate, share; };
 
 // Waves a SIMD asked of the compiler: 4 (128 registers a lane) where that costs next to no spills, 3 for the forms with more sums; a gate per
 // element without biases runs best at what it takes by itself (11712 x 2048: 144 us of a training pass, 153 at 3, 180 at 4).
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(THREADS, THREADS > 512 ? THREADS / 256 : bwd_waves(
   int64_t r, step, end, gate = 0;
   if (MODE == SPLIT) {
     const int64_t g = blockIdx.x / pl.per_gate, j = blockIdx.x % pl.per_gate;
-    const int64_t share = (pl.rows_per_gate + pl.per_gate - 1) / pl.per_gate, r0 = g * pl.rows_per_gate;
+    const int64_t share = pl.share, r0 = g * pl.rows_per_gate;
     end = r0 + (share * (j + 1) < pl.rows_per_gate ? share * (j + 1) : pl.rows_per_gate);
     r = r0 + share * j + sub;
     step = per;

@@ -52,24 +52,33 @@ static BwdPlan bwd_plan(const mscl_res_norm_desc* d) {
   BwdPlan p;
   res_norm_team(d->C, &p.T, &p.wave, &p.nv);
   const int per = p.wave ? 256 / p.T : 1;
-  // blocks for 256 CUs of 16 waves (128 registers a lane); every block costs up to 4 C floats of column sums
-  const int target = p.wave ? 1024 : 4096 / (p.T / 64);
   p.rows_per_gate = (int)(d->gate ? d->rows_per_gate : d->rows);
   p.gates = (int)(d->rows / p.rows_per_gate);
   // Many short runs: a team each.  (24 M elements, bf16, C = 64 / 512 / 2048, a training pass, WHOLE against SPLIT: runs of 4 rows 129 / 128 /
   // 124 against 1335 / 270 / 207 us, 16 rows 113 / 110 / 112 against 384 / 138 / 134, 32 rows 128 / 119 / 124 against 235 / 125 / 129, 64 rows
   // 153 / 148 / 161 against 163 / 121 / 128.)  Few runs of any length leave most teams without one.
-  const int teams = target * per;
+  const int teams = (p.wave ? 1024 : 4096 / (p.T / 64)) * per;
   const bool many = p.gates >= 4 * teams || (p.rows_per_gate <= 32 && p.gates >= (teams / 2 < 1024 ? teams / 2 : 1024));
   p.mode = !d->gate ? SPLIT : p.rows_per_gate == 1 ? EACH1 : many ? WHOLE : SPLIT;
+  // As many blocks as the 256 CUs hold at once (every block costs up to 4 C floats of column sums, and a second round of a few blocks as much
+  // time as the first): 4 waves a SIMD or 3, as bwd_waves and THREADS of the form leave registers.
+  const bool four = p.T > 768 || (p.T <= 512 && p.mode == SPLIT && !d->b_post && !d->b_pre && d->C >= 8);
+  const int target = 256 * (p.wave ? (four ? 4 : 3) : (four ? 16 : 12) / (p.T / 64));
   if (p.mode != SPLIT) {
     p.per_gate = 1;
+    p.share = p.rows_per_gate;
     const int64_t need = cdiv64(p.gates, per);
     p.blocks = (int)(need < target ? need : target);
   } else {
-    int64_t pg = cdiv64(target, p.gates);
-    if (pg > cdiv64(p.rows_per_gate, per)) pg = cdiv64(p.rows_per_gate, per);
-    p.per_gate = (int)pg;
+    // blocks of a gate: the number that costs the fewest rounds of the CUs for its share of rows, more than one round only for a tenth
+    int64_t pg = target / p.gates > 1 ? target / p.gates : 1;
+    double cost = (double)cdiv64(pg * p.gates, target) / pg;
+    for (int rounds = 2; rounds <= 4; ++rounds) {
+      const int64_t more = (int64_t)rounds * target / p.gates;
+      if (more > pg && (double)rounds / more < 0.9 * cost) { pg = more; cost = (double)rounds / more; }
+    }
+    p.share = (int)(cdiv64(cdiv64(p.rows_per_gate, pg), per) * per);             // whole rounds of the block's teams
+    p.per_gate = (int)cdiv64(p.rows_per_gate, p.share);
     p.blocks = p.per_gate * p.gates;
   }
   return p;
