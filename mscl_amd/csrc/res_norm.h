@@ -612,13 +612,19 @@ void res_norm_fwd_types(const mscl_res_norm_desc& d, hipStream_t st) {
   int T, wave, nv;
   res_norm_team(d.C, &T, &wave, &nv);
   const int per = wave ? 256 / T : 1;
-  // each block takes its rows in one stretch: enough blocks for 32 waves a CU, but no stretch longer than four rows a team -- short enough
-  // that the last blocks end together (32768 x 2048, fp32 / bf16: 172 us with 16 rows a team, 161 with 8, 155 with 4, 158 with 2)
-  int64_t grid = wave ? 2048 : 8192 / (T / 64);
-  if (grid < cdiv64(d.rows, 4 * per)) grid = cdiv64(d.rows, 4 * per);
-  if (grid > cdiv64(d.rows, per)) grid = cdiv64(d.rows, per);
-  const int64_t share = cdiv64(cdiv64(d.rows, grid), per) * per;
-  grid = cdiv64(d.rows, share);
+  // Each block takes its rows in one stretch, s to a team: short, so that the last blocks end together (32768 x 2048, fp32 / bf16: 172 us with
+  // 16 rows a team, 161 with 8, 155 with 4, 158 with 2), or so long that all blocks are resident at once.  Of these the s is taken with the
+  // fewest row times: rounds of the resident blocks (part of one more where they overlap) times s and one for a block's start.  (Against blocks
+  // for 32 waves a CU at up to 4 rows: 1556 x 6040 fp32 / bf16, biases, 31 -> 22 us; 6696 x 3584 bf16 41 -> 36; 400 x 5000 12 -> 9.)
+  const int waves = nv == 1 && !(d.b_post || d.b_pre) ? 5 : 4;             // a SIMD, by registers
+  const int64_t resident = 256 * (wave ? waves : waves * 4 / (T / 64));
+  int64_t share = per;
+  double best = 1e30;
+  for (int s = 1; s <= (wave ? 8 : 16); ++s) {
+    const double n = (double)cdiv64(d.rows, s * per) / resident, whole = n <= 1.0 ? 1.0 : n + 0.5 < ceil(n) ? n + 0.5 : ceil(n);
+    if ((s <= 4 || n <= 1.0) && whole * (s + 1) < best) { best = whole * (s + 1); share = s * per; }
+  }
+  const int64_t grid = cdiv64(d.rows, share);
   if (wave) fwd_launch<XT, FT, 1, true>(d, T, (unsigned)grid, share, st);
   else if (nv == 1) fwd_launch<XT, FT, 1, false>(d, T, (unsigned)grid, share, st);
   else fwd_launch<XT, FT, 2, false>(d, T, (unsigned)grid, share, st);
@@ -655,11 +661,14 @@ int res_norm_bwd_types(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_
   else if (p.T <= 768) bwd_launch<XT, FT, 1, false, 768>(d, p, st);        // 168 registers a lane; 1024 lanes leave 128
   else bwd_launch<XT, FT, 1, false, 1024>(d, p, st);
   MSCL_LAUNCH_CHECK();
-  const int cols = d.C < 1024 ? 4 : 16;        // 3 M elements, a training pass, C = 64 / 1024: 36 / 49 us with 4 columns a block, 38 / 38 with 16
+  // few columns a block for narrow rows (few blocks), whole 64-byte segments for wide ones (C = 64 / 1024, 3 M elements, a training pass: 36 / 49 us
+  // with 4 columns, 38 / 38 with 16; this launch at C = 1000 / 768 / 568: 29 / 18 / 19 us with 4, 17 / 13 / 13 with 8, 18 / 13 / 17 with 16)
+  const int cols = d.C < 512 ? 4 : d.C < 1024 ? 8 : 16;
   int lanes = 1;
   if (d.gate && p.mode == SPLIT) while (lanes * 2 * p.gates <= 512 / cols && lanes * 2 <= p.per_gate) lanes *= 2;
   const dim3 grid((d.C + cols - 1) / cols);
   if (cols == 4) hipLaunchKernelGGL((res_norm_finish_kernel<FT, 4>), grid, dim3(512), 0, st, d, p, lanes);
+  else if (cols == 8) hipLaunchKernelGGL((res_norm_finish_kernel<FT, 8>), grid, dim3(512), 0, st, d, p, lanes);
   else hipLaunchKernelGGL((res_norm_finish_kernel<FT, 16>), grid, dim3(512), 0, st, d, p, lanes);
   MSCL_LAUNCH_CHECK();
   return 0;
