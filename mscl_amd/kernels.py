@@ -685,13 +685,17 @@ def res_norm_fwd(x, f=None, *, gate=None, gate_act='sigmoid', scale=None, post_n
     if gate is not None:
         gate = gate.contiguous()
     h = _empty(x, kind) if pre_norm is not None else None
-    stats = (None,) * 4                                  # mean_f, rstd_f, mean_y, rstd_y
+    stats, held = None, [None] * 4                       # mean_f, rstd_f, mean_y, rstd_y: four runs of one buffer
     if save:
         want = (post_norm == 'layer', post_norm is not None, pre_norm == 'layer', pre_norm is not None)
-        held = iter(torch.empty((sum(want), rows), dtype=torch.float32, device=x.device).unbind(0))
-        stats = [next(held) if w else None for w in want]
+        stats = torch.empty(sum(want) * rows, dtype=torch.float32, device=x.device)
+        at = stats.data_ptr()
+        for i in range(4):
+            if want[i]:
+                held[i] = at
+                at += 4 * rows
     d = lib.ResNormDesc(x.data_ptr(), _at(f), _at(gate), _at(scale), _at(w_post), _at(b_post), _at(w_pre), _at(b_pre),
-                        y.data_ptr() if f is not None else None, _at(h), _at(stats[0]), _at(stats[1]), _at(stats[2]), _at(stats[3]))
+                        y.data_ptr() if f is not None else None, _at(h), *held)
     d.rows, d.ld_x, d.ld_f, d.rows_per_gate, d.C, d.x_type, d.f_type = rows, ld_x, ld_f, per, C, _TYPE_CODE[x.dtype], _TYPE_CODE[kind]
     d.post, d.pre, d.gate_act, d.eps = NORMS[post_norm], NORMS[pre_norm], GATES[gate_act], eps
     if rows:
