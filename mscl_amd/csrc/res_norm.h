@@ -321,12 +321,16 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void res_norm_fwd_kernel(mscl_re
 enum { SPLIT = 0, WHOLE = 1, EACH1 = 2 };
 struct BwdPlan { int T, wave, nv, mode, per_gate, gates, blocks, rows_per_gate, share; };
 
-// Waves a SIMD asked of the compiler: 4 (128 registers a lane) where that costs next to no spills, 3 for the forms with more sums; a gate per
-// element without biases runs best at what it takes by itself (11712 x 2048: 144 us of a training pass, 153 at 3, 180 at 4).
+// Waves a SIMD of the backward kernel (512 registers a lane shared among them): 3, which most forms run in without spills (a training pass of
+// 24 M elements, C = 192: bf16 110 us at 4, 108 at 3; fp32 290 at 4, 206 at 3), 2 for those with more sums (a gate per element and biases,
+// C = 192: bf16 144 us at 3, 141 at 2; fp32 422 at 3, 253 at 2; fp32 / bf16 in whole gates of 8 rows 221 and 167; bf16 in whole gates 130 at 3, 143 at
+// 2).  A gate per element without biases takes what it needs by itself (5856 x 4096 bf16: 127 us, 143 when told 3).  More than 768 lanes: 4.
 // LEAN (past 8192 channels, 16 of them a lane, 1024 lanes): no prefetch, the per-channel vectors read again for every row -- registers.
-constexpr int bwd_waves(int mode, bool bias) { return mode == SPLIT && !bias ? 4 : mode == EACH1 && !bias ? 1 : 3; }
+constexpr int bwd_waves(int threads, int xt, int ft, int mode, bool bias) {
+  return threads > 768 ? 4 : threads <= 512 && ((mode == EACH1 && (ft == MSCL_F32 || bias)) || (mode == WHOLE && xt == MSCL_F32)) ? 2 : 3;
+}
 template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS, bool NARROW>
-__global__ __launch_bounds__(THREADS, THREADS > 512 ? THREADS / 256 : bwd_waves(MODE, BIAS)) void res_norm_bwd_kernel(mscl_res_norm_desc d, BwdPlan pl) {
+__global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ? 1 : bwd_waves(THREADS, XT, FT, MODE, BIAS)) void res_norm_bwd_kernel(mscl_res_norm_desc d, BwdPlan pl) {
   extern __shared__ float lds[];                    // wave teams: [256][8 NV] for the column sums of a block
   __shared__ float2 red[32];
   constexpr int NB = BIAS ? NV : 1;

@@ -61,9 +61,9 @@ static BwdPlan bwd_plan(const mscl_res_norm_desc* d) {
   const bool many = p.gates >= 4 * teams || (p.rows_per_gate <= 32 && p.gates >= (teams / 2 < 1024 ? teams / 2 : 1024));
   p.mode = !d->gate ? SPLIT : p.rows_per_gate == 1 ? EACH1 : many ? WHOLE : SPLIT;
   // As many blocks as the 256 CUs hold at once (every block costs up to 4 C floats of column sums, and a second round of a few blocks as much
-  // time as the first): 4 waves a SIMD or 3, as bwd_waves and THREADS of the form leave registers.
-  const bool four = p.T > 768 || (p.T <= 512 && p.mode == SPLIT && !d->b_post && !d->b_pre && d->C >= 8);
-  const int target = 256 * (p.wave ? (four ? 4 : 3) : (four ? 16 : 12) / (p.T / 64));
+  // time as the first).
+  const int waves = bwd_waves(p.wave ? 256 : p.T, d->x_type, d->f_type, p.mode, p.mode == WHOLE || d->b_post || d->b_pre || d->C < 8);
+  const int target = 256 * (p.wave ? waves : waves * 4 / (p.T / 64));
   if (p.mode != SPLIT) {
     p.per_gate = 1;
     p.share = p.rows_per_gate;
