@@ -326,12 +326,18 @@ struct BwdPlan { int T, wave, nv, mode, per_gate, gates, blocks, rows_per_gate, 
 // C = 192: bf16 144 us at 3, 141 at 2; fp32 422 at 3, 253 at 2; fp32 / bf16 in whole gates of 8 rows 221 and 167; bf16 in whole gates 130 at 3, 143 at
 // 2).  A gate per element without biases takes what it needs by itself (5856 x 4096 bf16: 127 us, 143 when told 3).  More than 768 lanes: 4.
 // LEAN (past 8192 channels, 16 of them a lane, 1024 lanes): no prefetch, the per-channel vectors read again for every row -- registers.
+// LATE (also most forms of more than 768 lanes): a row's loads begin with its work (2928 x 8192, a training pass: fp32 with a gate per element 374
+// us with the next row in flight and spills, 259 without; bf16, no gate, no spills, 107 and 112).
 constexpr int bwd_waves(int threads, int xt, int ft, int mode, bool bias) {
   return threads > 768 ? 4 : threads <= 512 && ((mode == EACH1 && (ft == MSCL_F32 || bias)) || (mode == WHOLE && xt == MSCL_F32)) ? 2 : 3;
 }
+// Column sums that the backward kernel keeps in LDS: all four, two where 16 channels a lane and biases would need 256 KB.  (2928 x 8192, a training
+// pass, in registers with spills and so: bf16 with biases 181 / 117 us, with a gate per element as well 285 / 182.)
+constexpr int bwd_in_lds(int nv, int threads, bool bias) { return threads <= 768 ? 0 : nv == 2 && bias ? 2 : 4; }
+template <int K> struct Sum { static constexpr int value = K; };
 template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS, bool NARROW>
 __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ? 1 : bwd_waves(THREADS, XT, FT, MODE, BIAS)) void res_norm_bwd_kernel(mscl_res_norm_desc d, BwdPlan pl) {
-  extern __shared__ float lds[];                    // wave teams: [256][8 NV] for the column sums of a block
+  extern __shared__ float lds[];                    // wave teams: [256][8 NV] for the column sums of a block; more than 768 lanes: held()
   __shared__ float2 red[32];
   constexpr int NB = BIAS ? NV : 1;
   const int T = pl.T;
@@ -373,8 +379,8 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
     if (d.f && d.post) { if (layer1) sd[0] = d.mean_f[at]; sd[1] = d.rstd_f[at]; }
     if (d.dh) { if (layer2) sd[2] = d.mean_y[at]; sd[3] = d.rstd_y[at]; }
   };
-  constexpr bool LEAN = NV > 1;
-  if (!LEAN && r < end) fetch(r);
+  constexpr bool LEAN = NV > 1, LATE = LEAN || (THREADS > 768 && !(MODE == SPLIT && (!BIAS || XT != MSCL_F32)));
+  if (!LATE && r < end) fetch(r);
 
   float sw[NV][8], sb[NB][8], w2[NV][8], a[NV][8];
   float U1[NV][8] = {}, U2[NB][8] = {}, T1[NV][8] = {}, T2[NB][8] = {}, t1[MODE == WHOLE ? NV : 1][8] = {}, t2[MODE == WHOLE ? NB : 1][8] = {};
@@ -399,9 +405,29 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
   }
   int64_t loaded = -1;
 
+  // Column sum K += f.  Blocks of more than 768 lanes have 128 registers a lane: there the sums K < IN_LDS live in LDS, 16 bytes a lane at a time.
+  constexpr int IN_LDS = bwd_in_lds(NV, THREADS, BIAS);
+  auto held = [&](int k, int q, int h) -> float4& { return ((float4*)lds)[(((BIAS ? k : k / 2) * NV + q) * 2 + h) * T + lane]; };
+  auto add = [&](auto K, auto& sum, auto f) {
+    if constexpr (K.value < IN_LDS) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float4 v = held(K.value, q, h);
+          v.x += f(q, 4 * h); v.y += f(q, 4 * h + 1); v.z += f(q, 4 * h + 2); v.w += f(q, 4 * h + 3);
+          held(K.value, q, h) = v;
+        }
+    } else EACH sum[q][i] += f(q, i);
+  };
+  if (IN_LDS)
+    for (int k = 0; k < IN_LDS; k += BIAS ? 1 : 2)
+      for (int j = 0; j < 2 * NV; ++j) held(k, j / 2, j % 2) = make_float4(0.f, 0.f, 0.f, 0.f);         // a lane's own, no barrier
+
   while (r < end) {
     float x[NV][8], n[NV][8], t[NV][8], g[NV][8];
-    if (LEAN) { fetch(r); vectors(); }
+    if (LATE) fetch(r);
+    if (LEAN) vectors();
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       unpack<XT>(ux[q], x[q]);
@@ -412,7 +438,7 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
     }
     const float mu1 = sd[0], r1 = sd[1], mu2 = sd[2], r2 = sd[3];
     const int64_t next = after(r);
-    if (!LEAN && next < end) fetch(next);
+    if (!LATE && next < end) fetch(next);
     if (!d.dy) EACH t[q][i] = 0.f;
     float slope[MODE == EACH1 ? NV : 1][8];
     if constexpr (MODE == EACH1) {
@@ -430,13 +456,10 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
       if (d.dh) EACH x[q][i] += a[q][i] * (BIAS ? sw[q][i] * n[q][i] + sb[BIAS ? q : 0][i] : sw[q][i] * n[q][i]);        // y
     }
     if (d.dh) {
-      EACH {
-        const float yh = (x[q][i] - mu2) * r2;
-        x[q][i] = yh;
-        U1[q][i] += g[q][i] * yh;
-        if (BIAS) U2[BIAS ? q : 0][i] += g[q][i];
-        g[q][i] *= w2[q][i];
-      }
+      EACH x[q][i] = (x[q][i] - mu2) * r2;          // yhat
+      add(Sum<0>(), U1, [&](int q, int i) { return g[q][i] * x[q][i]; });
+      if constexpr (BIAS) add(Sum<1>(), U2, [&](int q, int i) { return g[q][i]; });
+      EACH g[q][i] *= w2[q][i];
       const float c1 = c.sum([&](int q, int i) { return g[q][i] * x[q][i]; });
       const float c0 = layer2 ? c.sum([&](int q, int i) { return g[q][i]; }) : 0.f;
       const float2 s = team.sum2(c1, c0, layer2);
@@ -445,18 +468,17 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
     }
     if (d.dx) c.template store<XT>(d.dx, r * d.C, t);
     if (d.f) {
-      EACH {
-        const float ti = t[q][i], tn = ti * n[q][i];
-        if (MODE == EACH1) {
-          T1[q][i] += a[q][i] * tn;
-          if (BIAS) T2[BIAS ? q : 0][i] += a[q][i] * ti;
-          slope[MODE == EACH1 ? q : 0][i] *= (BIAS ? sw[q][i] * tn + sb[BIAS ? q : 0][i] * ti : sw[q][i] * tn);
-        } else {
-          T1[q][i] += tn;
-          if (BIAS) T2[BIAS ? q : 0][i] += ti;
-        }
-        t[q][i] = ti * a[q][i] * sw[q][i];
+      if constexpr (MODE == EACH1) {
+        add(Sum<2>(), T1, [&](int q, int i) { return a[q][i] * (t[q][i] * n[q][i]); });
+        if constexpr (BIAS) add(Sum<3>(), T2, [&](int q, int i) { return a[q][i] * t[q][i]; });
+        EACH slope[q][i] *= BIAS ? sw[q][i] * (t[q][i] * n[q][i]) + sb[BIAS ? q : 0][i] * t[q][i] : sw[q][i] * (t[q][i] * n[q][i]);
+      } else if constexpr (MODE == SPLIT) {
+        add(Sum<2>(), T1, [&](int q, int i) { return t[q][i] * n[q][i]; });
+        if constexpr (BIAS) add(Sum<3>(), T2, [&](int q, int i) { return t[q][i]; });
+      } else {
+        EACH { T1[q][i] += t[q][i] * n[q][i]; T2[BIAS ? q : 0][i] += t[q][i]; }
       }
+      EACH t[q][i] = t[q][i] * a[q][i] * sw[q][i];
       if constexpr (MODE == EACH1) { if (d.dgate) c.template store<FT>(d.dgate, r * d.C, slope); }
       if (d.df) {
         if (d.post) {
@@ -472,12 +494,11 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
         if (next != r + 1 || next >= end || pl.rows_per_gate == 1) {        // the gate's last row
           c.template load<FT>(d.gate, gate * d.C, x);
           act_row<true, NV>(d.gate_act, x, n);
+          add(Sum<2>(), t1, [&](int q, int i) { return a[q][i] * T1[q][i]; });
+          add(Sum<3>(), t2, [&](int q, int i) { return a[q][i] * T2[BIAS ? q : 0][i]; });
           EACH {
-            const float s1 = T1[q][i], s2 = BIAS ? T2[BIAS ? q : 0][i] : 0.f;
-            t1[q][i] += a[q][i] * s1;
-            T1[q][i] = 0.f;
-            if (BIAS) { t2[BIAS ? q : 0][i] += a[q][i] * s2; T2[BIAS ? q : 0][i] = 0.f; }
-            x[q][i] = n[q][i] * (BIAS ? sw[q][i] * s1 + sb[BIAS ? q : 0][i] * s2 : sw[q][i] * s1);
+            x[q][i] = n[q][i] * (sw[q][i] * T1[q][i] + sb[BIAS ? q : 0][i] * T2[BIAS ? q : 0][i]);
+            T1[q][i] = T2[BIAS ? q : 0][i] = 0.f;
           }
           if (d.dgate) c.template store<FT>(d.dgate, gate * d.C, x);
           gate += step;
@@ -494,7 +515,16 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
     if (!BIAS && (k & 1)) continue;
     if (k < 2 ? !d.dh : !d.f) continue;             // block-uniform
     float v[NV][8];
-    EACH v[q][i] = k == 0 ? U1[q][i] : k == 1 ? U2[BIAS ? q : 0][i] : k == 2 ? (MODE == WHOLE ? t1[MODE == WHOLE ? q : 0][i] : T1[q][i])
+    if (k < IN_LDS) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 u = held(k, q, h);
+          v[q][4 * h] = u.x; v[q][4 * h + 1] = u.y; v[q][4 * h + 2] = u.z; v[q][4 * h + 3] = u.w;
+        }
+    } else
+      EACH v[q][i] = k == 0 ? U1[q][i] : k == 1 ? U2[BIAS ? q : 0][i] : k == 2 ? (MODE == WHOLE ? t1[MODE == WHOLE ? q : 0][i] : T1[q][i])
                  : (MODE == WHOLE ? t2[MODE == WHOLE && BIAS ? q : 0][i] : T2[BIAS ? q : 0][i]);
     if (!WAVE) { c.template store<MSCL_F32>(out + (int64_t)k * d.C, 0, v); continue; }
     __syncthreads();
@@ -635,7 +665,13 @@ void res_norm_fwd_types(const mscl_res_norm_desc& d, hipStream_t st) {
 }
 template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS, bool NARROW = false>
 static void bwd_go(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
-  hipLaunchKernelGGL((res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), dim3(p.blocks), dim3(WAVE ? 256 : p.T), WAVE ? 256 * 8 * NV * 4 : 0, st, d, p);
+  constexpr int IN_LDS = bwd_in_lds(NV, THREADS, BIAS);
+  const int bytes = WAVE ? 256 * 8 * NV * 4 : IN_LDS / (BIAS ? 1 : 2) * NV * 32 * p.T;
+  if constexpr (IN_LDS) {
+    static bool attr = false;
+    if (!attr) { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024); attr = true; }
+  }
+  hipLaunchKernelGGL((res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), dim3(p.blocks), dim3(WAVE ? 256 : p.T), bytes, st, d, p);
 }
 template <int XT, int FT, int NV, bool WAVE, int THREADS>
 static void bwd_launch(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
