@@ -668,8 +668,13 @@ static void bwd_go(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st
   constexpr int IN_LDS = bwd_in_lds(NV, THREADS, BIAS);
   const int bytes = WAVE ? 256 * 8 * NV * 4 : IN_LDS / (BIAS ? 1 : 2) * NV * 32 * p.T;
   if constexpr (IN_LDS) {
-    static bool attr = false;
-    if (!attr) { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024); attr = true; }
+    static uint64_t told = 0;                         // a bit per device
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (!(told >> (dev & 63) & 1)) {
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
+      told |= (uint64_t)1 << (dev & 63);
+    }
   }
   hipLaunchKernelGGL((res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), dim3(p.blocks), dim3(WAVE ? 256 : p.T), bytes, st, d, p);
 }

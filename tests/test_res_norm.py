@@ -231,6 +231,16 @@ def test_gate_runs(rows, C, gates, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('vecs', [VECS, ('scale', 'w_post', 'w_pre')])
+@pytest.mark.parametrize('gates', [0, 2, 150, 300])
+@pytest.mark.parametrize('C', [5000, 6144, 6145, 7000, 8191, 9001])
+def test_wide_rows(C, gates, vecs, dev):
+    """a block of 9 .. 16 waves a row, column sums in registers and in LDS: no gate, long and short runs, a gate for every row"""
+    _check(_case(C + gates, 300, C, BF, BF, 'rms', 'layer', gates, 'sigmoid', vecs), dev)
+    _check(_case(C + gates + 1, 300, C, F, *((BF, 'layer', 'rms') if C % 2 else (F, 'rms', 'rms')), gates, 'tanh', vecs), dev)
+
+
+@pytest.mark.gpu
 def test_bit_reproducible_accumulating_and_partial(dev):
     from mscl_amd import kernels as K_
     c = _case(5, 3000, 96, BF, BF, 'layer', 'rms', 30)
