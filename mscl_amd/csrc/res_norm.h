@@ -332,12 +332,15 @@ constexpr int bwd_waves(int threads, int xt, int ft, int mode, bool bias) {
   return threads > 768 ? 4 : threads <= 512 && ((mode == EACH1 && (ft == MSCL_F32 || bias)) || (mode == WHOLE && xt == MSCL_F32)) ? 2 : 3;
 }
 // Column sums that the backward kernel keeps in LDS: all four, two where 16 channels a lane and biases would need 256 KB.  (2928 x 8192, a training
-// pass, in registers with spills and so: bf16 with biases 181 / 117 us, with a gate per element as well 285 / 182.)
-constexpr int bwd_in_lds(int nv, int threads, bool bias) { return threads <= 768 ? 0 : nv == 2 && bias ? 2 : 4; }
+// pass, in registers with spills and so: bf16 with biases 181 / 117 us, with a gate per element as well 285 / 182; 4800 x 5000 fp32, a gate per
+// element and biases 377 / 268, bf16 164 / 160, without gates 130 / 134.)
+constexpr int bwd_in_lds(int nv, int threads, int xt, int mode, bool bias) {
+  return threads > 768 ? (nv == 2 && bias ? 2 : 4) : threads > 512 && xt == MSCL_F32 && mode != SPLIT && bias ? 4 : 0;
+}
 template <int K> struct Sum { static constexpr int value = K; };
 template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS, bool NARROW>
 __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ? 1 : bwd_waves(THREADS, XT, FT, MODE, BIAS)) void res_norm_bwd_kernel(mscl_res_norm_desc d, BwdPlan pl) {
-  extern __shared__ float lds[];                    // wave teams: [256][8 NV] for the column sums of a block; more than 768 lanes: held()
+  extern __shared__ float lds[];                    // wave teams: [256][8 NV] for the column sums of a block; bwd_in_lds: held()
   __shared__ float2 red[32];
   constexpr int NB = BIAS ? NV : 1;
   const int T = pl.T;
@@ -405,8 +408,8 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
   }
   int64_t loaded = -1;
 
-  // Column sum K += f.  Blocks of more than 768 lanes have 128 registers a lane: there the sums K < IN_LDS live in LDS, 16 bytes a lane at a time.
-  constexpr int IN_LDS = bwd_in_lds(NV, THREADS, BIAS);
+  // Column sum K += f.  Where registers lack (bwd_in_lds) the sums K < IN_LDS live in LDS, 16 bytes a lane at a time.
+  constexpr int IN_LDS = bwd_in_lds(NV, THREADS, XT, MODE, BIAS);
   auto held = [&](int k, int q, int h) -> float4& { return ((float4*)lds)[(((BIAS ? k : k / 2) * NV + q) * 2 + h) * T + lane]; };
   auto add = [&](auto K, auto& sum, auto f) {
     if constexpr (K.value < IN_LDS) {
@@ -665,7 +668,7 @@ void res_norm_fwd_types(const mscl_res_norm_desc& d, hipStream_t st) {
 }
 template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS, bool NARROW = false>
 static void bwd_go(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
-  constexpr int IN_LDS = bwd_in_lds(NV, THREADS, BIAS);
+  constexpr int IN_LDS = bwd_in_lds(NV, THREADS, XT, MODE, BIAS);
   const int bytes = WAVE ? 256 * 8 * NV * 4 : IN_LDS / (BIAS ? 1 : 2) * NV * 32 * p.T;
   if constexpr (IN_LDS) {
     static uint64_t told = 0;                         // a bit per device
