@@ -325,7 +325,8 @@ struct BwdPlan { int T, wave, nv, mode, per_gate, gates, blocks, rows_per_gate, 
 // 24 M elements, C = 192: bf16 110 us at 4, 108 at 3; fp32 290 at 4, 206 at 3), 2 for those with more sums (a gate per element and biases,
 // C = 192: bf16 144 us at 3, 141 at 2; fp32 422 at 3, 253 at 2; fp32 / bf16 in whole gates of 8 rows 221 and 167; bf16 in whole gates 130 at 3, 143 at
 // 2).  A gate per element without biases takes what it needs by itself (5856 x 4096 bf16: 127 us, 143 when told 3).  More than 768 lanes: 4.
-// LEAN (past 8192 channels, 16 of them a lane, 1024 lanes): no prefetch, the per-channel vectors read again for every row -- registers.
+// LEAN (past 8192 channels, 16 of them a lane, 1024 lanes): no prefetch, the per-channel vectors read again for every row -- registers.  LAZY: each
+// where it is used (2000 x 12000, a training pass: bf16 313 -> 276 us, fp32 / bf16 392 -> 300; whole gates lose, 467 -> 567).
 // LATE (also most forms of more than 768 lanes): a row's loads begin with its work (2928 x 8192, a training pass: fp32 with a gate per element 374
 // us with the next row in flight and spills, 259 without; bf16, no gate, no spills, 107 and 112).
 constexpr int bwd_waves(int threads, int xt, int ft, int mode, bool bias) {
@@ -382,25 +383,28 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
     if (d.f && d.post) { if (layer1) sd[0] = d.mean_f[at]; sd[1] = d.rstd_f[at]; }
     if (d.dh) { if (layer2) sd[2] = d.mean_y[at]; sd[3] = d.rstd_y[at]; }
   };
-  constexpr bool LEAN = NV > 1, LATE = LEAN || (THREADS > 768 && !(MODE == SPLIT && (!BIAS || XT != MSCL_F32)));
+  constexpr bool LEAN = NV > 1, LAZY = LEAN && MODE != WHOLE, LATE = LEAN || (THREADS > 768 && !(MODE == SPLIT && (!BIAS || XT != MSCL_F32)));
   if (!LATE && r < end) fetch(r);
 
   float sw[NV][8], sb[NB][8], w2[NV][8], a[NV][8];
   float U1[NV][8] = {}, U2[NB][8] = {}, T1[NV][8] = {}, T2[NB][8] = {}, t1[MODE == WHOLE ? NV : 1][8] = {}, t2[MODE == WHOLE ? NB : 1][8] = {};
-  auto vectors = [&] {
-    if (d.f) {
-      float s[NV][8];
-      c.load_vec(d.scale, 1.f, s);
-      c.load_vec(d.w_post, 1.f, sw);
-      EACH sw[q][i] *= s[q][i];
-      if constexpr (BIAS) {
-        c.load_vec(d.b_post, 0.f, sb);
-        EACH sb[q][i] *= s[q][i];
-      }
+  auto post_vectors = [&] {
+    if (LAZY) asm volatile("" ::: "memory");         // not before the values of the step above are done with
+    float s[NV][8];
+    c.load_vec(d.scale, 1.f, s);
+    c.load_vec(d.w_post, 1.f, sw);
+    EACH sw[q][i] *= s[q][i];
+    if constexpr (BIAS) {
+      c.load_vec(d.b_post, 0.f, sb);
+      EACH sb[q][i] *= s[q][i];
     }
-    if (d.dh) c.load_vec(d.w_pre, 1.f, w2);
   };
-  if (!LEAN) vectors();
+  auto pre_vectors = [&] {
+    if (LAZY) asm volatile("" ::: "memory");
+    c.load_vec(d.w_pre, 1.f, w2);
+  };
+  if (!LEAN && d.f) post_vectors();
+  if (!LEAN && d.dh) pre_vectors();
   EACH a[q][i] = 1.f;
   if (MODE == SPLIT && d.gate) {
     c.template load<FT>(d.gate, gate * d.C, a);
@@ -430,7 +434,7 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
   while (r < end) {
     float x[NV][8], n[NV][8], t[NV][8], g[NV][8];
     if (LATE) fetch(r);
-    if (LEAN) vectors();
+    if (LEAN && !LAZY) { if (d.f) post_vectors(); if (d.dh) pre_vectors(); }
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       unpack<XT>(ux[q], x[q]);
@@ -456,12 +460,14 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
     }
     if (d.f) {
       if (d.post) EACH n[q][i] = (n[q][i] - mu1) * r1;
+      if (LAZY && d.dh) post_vectors();
       if (d.dh) EACH x[q][i] += a[q][i] * (BIAS ? sw[q][i] * n[q][i] + sb[BIAS ? q : 0][i] : sw[q][i] * n[q][i]);        // y
     }
     if (d.dh) {
       EACH x[q][i] = (x[q][i] - mu2) * r2;          // yhat
       add(Sum<0>(), U1, [&](int q, int i) { return g[q][i] * x[q][i]; });
       if constexpr (BIAS) add(Sum<1>(), U2, [&](int q, int i) { return g[q][i]; });
+      if (LAZY) pre_vectors();
       EACH g[q][i] *= w2[q][i];
       const float c1 = c.sum([&](int q, int i) { return g[q][i] * x[q][i]; });
       const float c0 = layer2 ? c.sum([&](int q, int i) { return g[q][i]; }) : 0.f;
@@ -471,6 +477,7 @@ __global__ __launch_bounds__(THREADS, THREADS <= 512 && MODE == EACH1 && !BIAS ?
     }
     if (d.dx) c.template store<XT>(d.dx, r * d.C, t);
     if (d.f) {
+      if (LAZY) post_vectors();
       if constexpr (MODE == EACH1) {
         add(Sum<2>(), T1, [&](int q, int i) { return a[q][i] * (t[q][i] * n[q][i]); });
         if constexpr (BIAS) add(Sum<3>(), T2, [&](int q, int i) { return a[q][i] * t[q][i]; });

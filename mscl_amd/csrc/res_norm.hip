@@ -57,8 +57,10 @@ static BwdPlan bwd_plan(const mscl_res_norm_desc* d) {
   // Many short runs: a team each.  (24 M elements, bf16, C = 64 / 512 / 2048, a training pass, WHOLE against SPLIT: runs of 4 rows 129 / 128 /
   // 124 against 1335 / 270 / 207 us, 16 rows 113 / 110 / 112 against 384 / 138 / 134, 32 rows 128 / 119 / 124 against 235 / 125 / 129, 64 rows
   // 153 / 148 / 161 against 163 / 121 / 128.)  Few runs of any length leave most teams without one.
+  // Past 8192 channels WHOLE has the most spills and is for very many gates alone (SPLIT's sums of each gate are 16 bytes a channel): 2000 x 12000
+  // bf16, runs of 8 / 2 rows 467 / 578 us, SPLIT 294 / 399.
   const int teams = (p.wave ? 1024 : 4096 / (p.T / 64)) * per;
-  const bool many = p.gates >= 4 * teams || (p.rows_per_gate <= 32 && p.gates >= (teams / 2 < 1024 ? teams / 2 : 1024));
+  const bool many = p.gates >= 4 * teams || (p.nv == 1 && p.rows_per_gate <= 32 && p.gates >= (teams / 2 < 1024 ? teams / 2 : 1024));
   p.mode = !d->gate ? SPLIT : p.rows_per_gate == 1 ? EACH1 : many ? WHOLE : SPLIT;
   // As many blocks as the 256 CUs hold at once (every block costs up to 4 C floats of column sums, and a second round of a few blocks as much
   // time as the first).

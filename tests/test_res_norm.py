@@ -241,6 +241,17 @@ def test_wide_rows(C, gates, vecs, dev):
 
 
 @pytest.mark.gpu
+def test_whole_gates_past_8192_channels(dev):
+    """so many short runs that a team takes whole gates there too; the 64-bit reference runs on the GPU for its size"""
+    c = _case(77, 3680, 8200, BF, BF, 'rms', 'layer', 1840)
+    t, g, y, h, saved, grads = _run(c, dev)
+    want = _want(c, g)
+    for k, v in dict(grads, y=y, h=h).items():
+        val, mag = want[k if k in ('y', 'h') else 'd' + k]
+        _close(v, (val.cpu(), mag.cpu()), k)
+
+
+@pytest.mark.gpu
 def test_bit_reproducible_accumulating_and_partial(dev):
     from mscl_amd import kernels as K_
     c = _case(5, 3000, 96, BF, BF, 'layer', 'rms', 30)
