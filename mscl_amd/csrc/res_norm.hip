@@ -54,9 +54,9 @@ static BwdPlan bwd_plan(const mscl_res_norm_desc* d) {
   const int per = p.wave ? 256 / p.T : 1;
   p.rows_per_gate = (int)(d->gate ? d->rows_per_gate : d->rows);
   p.gates = (int)(d->rows / p.rows_per_gate);
-  // Many short runs: a team each.  (24 M elements, bf16, C = 64 / 512 / 2048, a training pass, WHOLE against SPLIT: runs of 4 rows 129 / 128 /
-  // 124 against 1335 / 270 / 207 us, 16 rows 113 / 110 / 112 against 384 / 138 / 134, 32 rows 128 / 119 / 124 against 235 / 125 / 129, 64 rows
-  // 153 / 148 / 161 against 163 / 121 / 128.)  Few runs of any length leave most teams without one.
+  // Many short runs: a team each.  (24 M elements, bf16, C = 64 / 512 / 2048, a training pass, WHOLE against SPLIT: runs of 8 rows 121 / 112 /
+  // 114 against 725 / 208 / 150 us, 16 rows 113 / 110 / 113 against 398 / 151 / 129, 32 rows 131 / 119 / 118 against 233 / 123 / 117; 64 rows, C = 64 /
+  // 192: 154 / 161 against 159 / 127.)  Few runs of any length leave most teams without one.
   // Past 8192 channels WHOLE has the most spills and is for very many gates alone (SPLIT's sums of each gate are 16 bytes a channel): 2000 x 12000
   // bf16, runs of 8 / 2 rows 467 / 578 us, SPLIT 294 / 399.
   const int teams = (p.wave ? 1024 : 4096 / (p.T / 64)) * per;
