@@ -147,6 +147,12 @@ template <int NV, bool NARROW> struct Cols {
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
   return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
 }
+// A row of 16 lanes to one value, the same bits in each of them: every step adds the two halves of a pair in both halves (half mirror: the
+// other quad of 8 lanes), and an addition commutes.  A rotation by a quad would add four quads in two different orders, and the lanes that
+// share a channel would store different bits for it (9 waves or more: the last bit of 1 / deviation in a tenth of the rows).
+__device__ __forceinline__ float row16_same(float v) {
+  return dpp_add<0x128>(dpp_add<0x141>(dpp_add<0x4E>(dpp_add<0xB1>(v))));
+}
 template <bool WAVE> struct Team {
   int T;
   float2* red;          // block teams: [2][16]
@@ -173,7 +179,7 @@ template <bool WAVE> struct Team {
     if ((threadIdx.x & 63) == 0) s[w] = make_float2(a, b);
     __syncthreads();
     const float2 t = l < nw ? s[l] : make_float2(0.f, 0.f);          // every 16 lanes add the (at most 16) waves' values
-    return make_float2(row16_sum(t.x), want_b ? row16_sum(t.y) : 0.f);
+    return make_float2(row16_same(t.x), want_b ? row16_same(t.y) : 0.f);
   }
   __device__ __forceinline__ float sum(float a) { return sum2(a, 0.f, false).x; }
 };
