@@ -184,8 +184,11 @@ template <bool WAVE> struct Team {
   __device__ __forceinline__ float sum(float a) { return sum2(a, 0.f, false).x; }
 };
 
-// exp(x) for x <= 0 to about 2 ulp: the rounding of x log2(e) is put back to first order
+// exp(x) for x <= 0 to about 2 ulp: the rounding of x log2(e) is put back to first order.  It is 0 from -104 on (and flushed below 2^-126), so
+// -150 stands for all that is lower: a shut gate has the type's lowest value or -inf, whose product overflows and leaves no correction.  (Not
+// fmaxf, which would take a NaN for a shut gate.)
 __device__ __forceinline__ float exp_neg(float x) {
+  x = x < -150.f ? -150.f : x;
   const float t = x * 1.44269504f, lo = fmaf(x, 1.92596303e-8f, fmaf(x, 1.44269504f, -t));
   const float e = __builtin_amdgcn_exp2f(t);
   return fmaf(e, lo * 0.693147181f, e);

@@ -8,12 +8,13 @@ import torch
 
 
 def _act(g, act):
+    # slopes from the exponential: a (1 - a) and 1 - a^2 cancel where a gate saturates
     if act == 'sigmoid':
-        a = 1 / (1 + torch.exp(-g))
-        return a, a * (1 - a)
+        e = torch.exp(-g.abs())
+        return 1 / (1 + torch.exp(-g)), e / (1 + e) ** 2
     if act == 'tanh':
-        a = torch.tanh(g)
-        return a, 1 - a * a
+        e = torch.exp(-2 * g.abs())
+        return torch.tanh(g), 4 * e / (1 + e) ** 2
     return g, torch.ones_like(g)
 
 

@@ -1,0 +1,82 @@
+"""Calls of the residual norm at the ends of their range: gates that are shut or open for good, rows of many waves, maps without rows,
+entries of the C interface that ask for a gradient nothing computes, and the module under autograd's own tools."""
+import ctypes
+import gc
+import weakref
+
+import pytest
+import torch
+
+from oracle import res_norm as oracle
+
+U, K = 2.0 ** -24, 512                   # as derived in test_res_norm.py
+BF, H, F = torch.bfloat16, torch.float16, torch.float32
+VECS = ('scale', 'w_post', 'b_post', 'w_pre', 'b_pre')
+
+
+def _close(got, want, what, floor=0.0):
+    val, mag = want
+    g = got.detach().cpu().double()
+    tol = torch.finfo(got.dtype).eps / 2 * val.abs() + K * U * mag + floor
+    if got.dtype == H:
+        tol = tol + 2.0 ** -25           # below 2^-14 fp16 has a fixed step of 2^-24
+    assert g.shape == val.shape and bool(torch.isfinite(g).all()), what
+    worst = float(((g - val).abs() / tol.clamp_min(1e-40)).max()) if g.numel() else 0.0
+    assert worst <= 1, (what, worst)
+
+
+# ------------------------------------------------------------------------------------------------------------ gates shut and open
+@pytest.mark.parametrize('act', ['sigmoid', 'tanh'])
+def test_oracle_gate_ends(act):
+    """values and slopes where 1 - a rounds to 0 or e^g overflows, against the exponential series' leading term"""
+    g = torch.tensor([float('inf'), float('-inf'), 3.3e38, -3.3e38, 1e4, -1e4, 40.0, -40.0], dtype=torch.float64)
+    a, slope = oracle._act(g, act)
+    low = 0.0 if act == 'sigmoid' else -1.0
+    e = torch.exp(torch.tensor(-40.0 if act == 'sigmoid' else -80.0, dtype=torch.float64))
+    assert a[:6].tolist() == [1.0, low] * 3 and slope[:6].tolist() == [0.0] * 6
+    assert bool((slope[6:] / (e if act == 'sigmoid' else 4 * e) - 1).abs().max() < 1e-15)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('xt,ft', [(BF, BF), (H, H), (F, F), (F, BF)])
+@pytest.mark.parametrize('rows,C,gates', [(24, 48, 24), (96, 48, 3), (8192, 16, 1024), (6, 5000, 6), (6, 5000, 2), (3, 9000, 3)])
+@pytest.mark.parametrize('act', ['sigmoid', 'tanh'])
+def test_saturated_gates(act, rows, C, gates, xt, ft, dev):
+    """Logits of +-inf, of the type's largest and lowest value, and every order of magnitude down to 1, among ordinary ones: for each row, for
+    long and for short runs of rows.  The exponential flushes what lies below 2^-126, so a value or slope of a gate is off by that much
+    besides; the terms that it multiplies are summed to less than 2^10 here: 2^-116."""
+    from mscl_amd import kernels as K_
+    gen = torch.Generator().manual_seed(rows + C + gates)
+    ends = torch.tensor([float('inf'), float('-inf'), torch.finfo(ft).max, torch.finfo(ft).min] +
+                        [s * m for s in (1, -1) for m in (6e4, 1e4, 1e3, 150.0, 104.0, 103.0, 89.0, 87.0, 60.0, 30.0, 17.0, 9.0, 4.0, 1.0)])
+    gate = 2 * torch.randn(gates, C, generator=gen)
+    pick = torch.randint(0, 2 * len(ends), (gates, C), generator=gen)
+    gate = torch.where(pick < len(ends), ends[pick.clamp_max(len(ends) - 1)], gate).to(ft)
+    assert bool(torch.isinf(gate).any())
+    x, f = torch.randn(rows, C, generator=gen).to(xt), torch.randn(rows, C, generator=gen).to(ft)
+    dy, dh = torch.randn(rows, C, generator=gen).to(xt), torch.randn(rows, C, generator=gen).to(ft)
+    vec = {k: torch.randn(C, generator=gen) * 0.2 + (1.0 if k.startswith('w') else 0.3) for k in VECS}
+    d = {k: v.double() for k, v in vec.items()}
+    want = oracle.run(x.double(), f.double(), gate.double(), act, d['scale'], 'rms', d['w_post'], d['b_post'], 'layer', d['w_pre'], d['b_pre'], 1e-6,
+                      dy.double(), dh.double())
+    y, h, saved = K_.res_norm_fwd(x.to(dev), f.to(dev), gate=gate.to(dev), gate_act=act, post_norm='rms', pre_norm='layer', save=True,
+                                  **{k: v.to(dev) for k, v in vec.items()})
+    got = dict(K_.res_norm_bwd(saved, dy.to(dev), dh.to(dev)), y=y, h=h)
+    for k, v in got.items():
+        _close(v, want[k if k in ('y', 'h') else 'd' + k], (k, act), 2.0 ** -116)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ['sigmoid', 'tanh'])
+def test_nan_gates_stay_nan(act, dev):
+    """a logit that is no number is not taken for a shut gate"""
+    from mscl_amd import kernels as K_
+    x = torch.randn(6, 64, device=dev)
+    gate = torch.zeros(6, 64, device=dev)
+    gate[2, 5] = float('nan')
+    for g, rows in ((gate, [2]), (gate[1:4:2].contiguous(), []), (gate[2:4].contiguous(), [0, 1, 2])):
+        y, _, saved = K_.res_norm_fwd(x, x, gate=g, gate_act=act, save=True)
+        bad = torch.isnan(y)
+        assert sorted(bad.nonzero()[:, 0].tolist()) == rows and bool((bad.nonzero()[:, 1] == 5).all())
+        out = K_.res_norm_bwd(saved, x)
+        assert torch.equal(torch.isnan(out['gate']), torch.isnan(g))
