@@ -744,6 +744,8 @@ def res_norm_bwd(saved, dy=None, dh=None, into=None, need=None):
             src = getattr(saved, k)
             out[k] = _empty(src, src.dtype)
     if rows == 0:
+        if 'gate' in out:                                # (n, C) gates of no rows
+            out['gate'].zero_()
         return out
     d = lib.ResNormDesc.from_buffer_copy(d)
     d.dy, d.dh, d.accumulate = _at(dy), _at(dh), int(into is not None)

@@ -80,3 +80,19 @@ def test_nan_gates_stay_nan(act, dev):
         assert sorted(bad.nonzero()[:, 0].tolist()) == rows and bool((bad.nonzero()[:, 1] == 5).all())
         out = K_.res_norm_bwd(saved, x)
         assert torch.equal(torch.isnan(out['gate']), torch.isnan(g))
+
+
+# ------------------------------------------------------------------------------------------------------------ no rows
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [F, BF])
+def test_gates_of_an_empty_batch_get_zero_gradients(dtype, dev):
+    """gates may outnumber the rows of an empty batch: their gradient is a sum over no rows"""
+    from mscl_amd import kernels as K_
+    x = torch.zeros(0, 16, dtype=dtype, device=dev)
+    gate, w = torch.randn(3, 16, device=dev).to(dtype), torch.ones(16, device=dev)
+    _, _, saved = K_.res_norm_fwd(x, x, gate=gate, scale=w, save=True)
+    for _ in range(3):
+        held = [torch.full((3, 16), float('nan'), dtype=dtype, device=dev) for _ in range(8)]        # what the allocator hands out next
+        del held
+        g = K_.res_norm_bwd(saved, x)
+        assert g['gate'].shape == gate.shape and not g['gate'].any() and not g['scale'].any() and g['x'].shape == x.shape
