@@ -11,6 +11,7 @@ import ctypes
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 from . import lib
@@ -979,6 +980,7 @@ class _ResNormFn(torch.autograd.Function):
         return h if f is None else y if h is None else (y, h)
 
     @staticmethod
+    @once_differentiable                 # (kernels leave no graph: a second derivative would lack their terms)
     def backward(ctx, *grads):
         ctx.saved_tensors
         if torch.cuda.is_current_stream_capturing() != ctx.capturing:

@@ -96,3 +96,31 @@ def test_gates_of_an_empty_batch_get_zero_gradients(dtype, dev):
         del held
         g = K_.res_norm_bwd(saved, x)
         assert g['gate'].shape == gate.shape and not g['gate'].any() and not g['scale'].any() and g['x'].shape == x.shape
+
+
+# ------------------------------------------------------------------------------------------------------------ the module
+def _module(dev, C=16, **kw):
+    from mscl_amd.arena import ParamArena
+    from mscl_amd.nn import ResNormHip
+    from mscl_amd.recognizers import bind_module
+    m = ResNormHip(C, 'rms', 'layer', scale=0.5, bias=True, **kw)
+    ar = ParamArena(dev)
+    plan = [(ar.add(n, p.shape), p) for n, p in m.named_parameters()]
+    ar.allocate(with_key=False)
+    for slot, p in plan:
+        v = ar.view('Q', slot)
+        v.copy_(p.data)
+        p.data, p.grad, p._mscl_slot = v, ar.view('G', slot), slot
+    bind_module(m, ar, False, m)
+    return m, ar
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused(dev):
+    """the backward pass is no graph of its own: differentiating through it would leave terms out"""
+    m, _ = _module(dev)
+    x, f = (torch.randn(5, 16, device=dev, requires_grad=True) for _ in range(2))
+    y, h = m(x, f)
+    g, = torch.autograd.grad((y * y).sum() + (h * h).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        torch.autograd.grad((g * g).sum() + (x * x).sum(), x)
