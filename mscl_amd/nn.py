@@ -11,7 +11,6 @@ import ctypes
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 from . import lib
@@ -966,6 +965,19 @@ class Conv1dK1Hip(nn.Module):
 
 
 # ------------------------------------------------------------------------------------------ residual norm
+class _Once(torch.autograd.Function):
+    """the gradients of a node that cannot be differentiated again, tied to all that they depend on: whoever differentiates through them
+    arrives here, also torch.autograd.grad, which walks only towards the tensors it is asked for (and so past torch's own once_differentiable)"""
+
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tuple(None if t is None else t.view_as(t) for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise MsclError('residual norm: its gradients are once_differentiable (the kernels leave no graph to differentiate again)')
+
+
 class _ResNormFn(torch.autograd.Function):
     """(y, h) of kernels.res_norm_fwd as one graph node; h alone without a branch.  The module's own gradients go straight into the arena."""
 
@@ -980,7 +992,6 @@ class _ResNormFn(torch.autograd.Function):
         return h if f is None else y if h is None else (y, h)
 
     @staticmethod
-    @once_differentiable                 # (kernels leave no graph: a second derivative would lack their terms)
     def backward(ctx, *grads):
         ctx.saved_tensors
         if torch.cuda.is_current_stream_capturing() != ctx.capturing:
@@ -996,7 +1007,10 @@ class _ResNormFn(torch.autograd.Function):
         out = K.res_norm_bwd(saved, dy, dh, into=mod._rt['grad'], need=need)
         for k in mod._live(saved.f is not None, dh is not None):
             mod._rt['slots'][k].touched = True
-        return out.get('x'), out.get('f'), out.get('gate'), None, None
+        made = out.get('x'), out.get('f'), out.get('gate')
+        if torch.is_grad_enabled():                      # create_graph=True
+            made = _Once.apply(3, *made, dy, dh, *ctx.saved_tensors)
+        return *made, None, None
 
 
 class ResNormHip(nn.Module):
@@ -1039,5 +1053,7 @@ class ResNormHip(nn.Module):
             return y, h
         if self._anchor is None or self._anchor.device != x.device:
             self._anchor = torch.zeros(1, device=x.device, requires_grad=True)
-        out = _ResNormFn.apply(x, f, gate, self._anchor, self)
+        # copies that the kernels need (gaps between rows that no stride describes) are made here, in autograd's sight
+        x, f = (t if t is None or t.is_contiguous() else K._rows_of(t, t.shape[-1])[0] for t in (x, f))
+        out = _ResNormFn.apply(x, f, gate if gate is None else gate.contiguous(), self._anchor, self)
         return (x, out) if f is None else out if self.pre is not None else (out, None)
