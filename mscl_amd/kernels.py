@@ -618,7 +618,31 @@ def _empty(t, dtype):
 
 class ResNormSaved:
     """what res_norm_bwd needs of a forward call"""
-    __slots__ = ('x', 'f', 'gate', 'vec', 'stats', 'desc', 'names', 'shape', 'kind')
+    __slots__ = ('x', 'f', 'gate', 'vec', 'stats', 'desc', 'names', 'shape', 'kind', 'stats_at')
+
+    def release(self):
+        """hands the tensors out (missing ones as None) and keeps only what describes them: for a keeper of its own, such as autograd's"""
+        out = self.x, self.f, self.gate, self.stats
+        self.x = self.f = self.gate = self.stats = None
+        return out
+
+    def restored(self, x, f, gate, stats):
+        """a whole one again from release()'s tensors, which may lie elsewhere and otherwise by now"""
+        s, d = ResNormSaved(), lib.ResNormDesc.from_buffer_copy(self.desc)
+        x, d.ld_x = _rows_of(x, d.C)
+        if f is not None:
+            f, d.ld_f = _rows_of(f, d.C)
+        if gate is not None:
+            gate = gate.contiguous()
+        stats = stats.contiguous()
+        d.x, d.f, d.gate = x.data_ptr(), _at(f), _at(gate)
+        for k in ('mean_f', 'rstd_f', 'mean_y', 'rstd_y'):
+            at = getattr(d, k)
+            if at:
+                setattr(d, k, at - self.stats_at + stats.data_ptr())
+        s.x, s.f, s.gate, s.stats, s.stats_at, s.desc = x, f, gate, stats, stats.data_ptr(), d
+        s.vec, s.names, s.shape, s.kind = self.vec, self.names, self.shape, self.kind
+        return s
 
 
 def _res_norm_check(x, f, gate, vec, post_norm, pre_norm, gate_act, eps):
@@ -704,7 +728,7 @@ def res_norm_fwd(x, f=None, *, gate=None, gate_act='sigmoid', scale=None, post_n
         return y, h, None
     saved = ResNormSaved()
     saved.x, saved.f, saved.gate, saved.vec, saved.stats, saved.desc = x, f, gate, vec, stats, d
-    saved.shape, saved.kind = x.shape, kind
+    saved.shape, saved.kind, saved.stats_at = x.shape, kind, stats.data_ptr()
     saved.names = [k for k, t in (('x', x), ('f', f), ('gate', gate)) if t is not None] + [k for k in _VECTORS if vec[k] is not None]
     return y, h, saved
 

@@ -984,8 +984,8 @@ class _ResNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, gate, anchor, mod):
         y, h, saved = K.res_norm_fwd(x, f, gate=gate, save=True, **mod._args(f is not None))
-        tensors = [t for t in (saved.x, saved.f, saved.gate) if t is not None]
-        ctx.save_for_backward(*tensors)                  # (its version check refuses a backward over inputs changed in place)
+        # autograd keeps the tensors, alone: its version check refuses a backward over inputs changed in place, its hooks may move them
+        ctx.save_for_backward(*saved.release())
         ctx.saved, ctx.mod = saved, mod
         ctx.capturing = torch.cuda.is_current_stream_capturing()
         ctx.set_materialize_grads(False)
@@ -993,10 +993,10 @@ class _ResNormFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        ctx.saved_tensors
+        kept = ctx.saved_tensors
         if torch.cuda.is_current_stream_capturing() != ctx.capturing:
             raise MsclError('residual norm: forward and backward belong into the same graph capture, or both outside of one')
-        saved, mod = ctx.saved, ctx.mod
+        saved, mod = ctx.saved.restored(*kept), ctx.mod
         if saved.f is None:
             dy, dh = None, grads[0]
         else:
@@ -1009,7 +1009,7 @@ class _ResNormFn(torch.autograd.Function):
             mod._rt['slots'][k].touched = True
         made = out.get('x'), out.get('f'), out.get('gate')
         if torch.is_grad_enabled():                      # create_graph=True
-            made = _Once.apply(3, *made, dy, dh, *ctx.saved_tensors)
+            made = _Once.apply(3, *made, dy, dh, *kept[:3])
         return *made, None, None
 
 

@@ -124,3 +124,51 @@ def test_second_derivatives_are_refused(dev):
     g, = torch.autograd.grad((y * y).sum() + (h * h).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match='once_differentiable'):
         torch.autograd.grad((g * g).sum() + (x * x).sum(), x)
+
+
+class _Offload:
+    """hooks that keep saved tensors on the host, densely packed"""
+
+    def __init__(self, dev):
+        self.dev, self.packed = dev, 0
+
+    def pack(self, t):
+        self.packed += 1
+        return t.to('cpu', copy=True).contiguous()
+
+    def unpack(self, t):
+        return t.to(self.dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('strided', [False, True])
+def test_saved_tensor_hooks_move_the_inputs(strided, dev):
+    """under saved-tensor hooks nothing but the hooks' copies stays; gradients are the same bits, also where a copy is laid out otherwise"""
+    torch.manual_seed(0)
+    shape = (40, 32) if strided else (40, 16)
+    x0, f0, gate0 = torch.randn(shape, device=dev), torch.randn(shape, device=dev), torch.randn(4, 16, device=dev)
+    dy, dh = torch.randn(40, 16, device=dev), torch.randn(40, 16, device=dev)
+    want = None
+    for hooked in (False, True):
+        m, ar = _module(dev)
+        x, f, gate = (t.clone().requires_grad_() for t in (x0, f0, gate0))
+        off = _Offload(dev)
+
+        def forward():
+            a, b, c = x * 1.0, f * 1.0, gate * 1.0
+            y, h = m(a[:, 8:24], b[:, 8:24], c) if strided else m(a, b, c)
+            return y, h, [weakref.ref(t) for t in (a, b, c)]
+        if hooked:
+            with torch.autograd.graph.saved_tensors_hooks(off.pack, off.unpack):
+                y, h, refs = forward()
+            gc.collect()
+            assert off.packed >= 3 and all(r() is None for r in refs)
+        else:
+            y, h, refs = forward()
+        torch.autograd.backward([y, h], [dy, dh], retain_graph=True)
+        got = [x.grad.clone(), f.grad.clone(), gate.grad.clone(), ar.G.clone()]
+        if want is not None:
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+        want = got
+        torch.autograd.backward([y, h], [dy, dh])           # a second pass over the same graph accumulates
+        assert torch.equal(x.grad, 2 * got[0]) and torch.equal(ar.G, 2 * got[3])
