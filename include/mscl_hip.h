@@ -460,7 +460,7 @@ int mscl_adamw_values(const uint8_t* m, const uint8_t* v, const uint8_t* exponen
  * (x_type, f_type) equal, or fp32 with a 16-bit f_type; per-channel vectors and statistics fp32.  C <= MSCL_RES_NORM_MAX_C, rows < 2^31.
  * The forward writes the statistics that are not NULL; the backward wants those of the norms it goes through, x and f as in the forward,
  * dy and / or dh, and writes the gradients that are not NULL -- per-channel ones added to what is there when accumulate != 0; those that
- * a missing f or dh keeps from having one are left alone.
+ * a missing f or dh keeps from having one are left alone, those of a bias or gate that is NULL are refused.
  * Deterministic.  The BatchNorm counterpart is mscl_bn_act_fwd / _bwd. */
 #define MSCL_NORM_RMS   1
 #define MSCL_NORM_LAYER 2

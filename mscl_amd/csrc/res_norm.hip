@@ -94,6 +94,7 @@ extern "C" int mscl_res_norm_bwd(const mscl_res_norm_desc* d, void* stream) {
   const int rc = res_norm_check(d);
   if (rc) return rc;
   if (!d->dy && !d->dh) return MSCL_E_ARG;
+  if ((d->db_post && !d->b_post) || (d->db_pre && !d->b_pre) || (d->dgate && !d->gate)) return MSCL_E_ARG;        // no sums are kept for these
   if ((d->dh && (!d->pre || !d->rstd_y || (d->pre == MSCL_NORM_LAYER && !d->mean_y)))) return MSCL_E_ARG;
   if (d->f && d->post && (!d->rstd_f || (d->post == MSCL_NORM_LAYER && !d->mean_f))) return MSCL_E_ARG;
   const BwdPlan p = bwd_plan(d);

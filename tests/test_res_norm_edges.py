@@ -172,3 +172,17 @@ def test_saved_tensor_hooks_move_the_inputs(strided, dev):
         want = got
         torch.autograd.backward([y, h], [dy, dh])           # a second pass over the same graph accumulates
         assert torch.equal(x.grad, 2 * got[0]) and torch.equal(ar.G, 2 * got[3])
+
+
+# ------------------------------------------------------------------------------------------------------------ C interface
+def test_gradients_without_their_input_are_refused():
+    """a bias gradient without that bias, or a gate gradient without a gate, is computed by no kernel: asked for, it is refused before any
+    launch"""
+    from mscl_amd import lib
+    d = lib.ResNormDesc(x=16, f=16, dy=16, dh=16, rstd_f=16, rstd_y=16, ws=16, rows=4, C=8, ld_x=8, ld_f=8, rows_per_gate=4, x_type=2, f_type=2,
+                        post=1, pre=1, eps=1e-6)
+    d.ws_floats = lib.call_raw('mscl_res_norm_ws', ctypes.byref(d))
+    for name in ('db_post', 'db_pre', 'dgate'):
+        e = lib.ResNormDesc.from_buffer_copy(d)
+        setattr(e, name, 16)
+        assert lib.call_raw('mscl_res_norm_bwd', ctypes.byref(e), None) == -1, name
