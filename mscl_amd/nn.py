@@ -1029,7 +1029,7 @@ class ResNormHip(nn.Module):
                     b_pre=0.0 if pre and bias else None)
         for name, v in fill.items():
             self.register_parameter(name, None if v is None else nn.Parameter(torch.full((channels,), float(v))))
-        self._rt = self._anchor = None
+        self._rt = None
 
     def extra_repr(self):
         return f'{self.channels}, post={self.post}, pre={self.pre}, gate_act={self.gate_act}, eps={self.eps}'
@@ -1051,9 +1051,12 @@ class ResNormHip(nn.Module):
         if not torch.is_grad_enabled():
             y, h, _ = K.res_norm_fwd(x, f, gate=gate, **self._args(f is not None))
             return y, h
-        if self._anchor is None or self._anchor.device != x.device:
-            self._anchor = torch.zeros(1, device=x.device, requires_grad=True)
         # copies that the kernels need (gaps between rows that no stride describes) are made here, in autograd's sight
         x, f = (t if t is None or t.is_contiguous() else K._rows_of(t, t.shape[-1])[0] for t in (x, f))
-        out = _ResNormFn.apply(x, f, gate if gate is None else gate.contiguous(), self._anchor, self)
+        # The parameters' gradients need the node also where no input does.  A leaf of the call's own: one that calls share has one accumulation
+        # node, which stays on the stream of the first call, and a capture that meets it while an eager graph lives waits on that stream.
+        anchor = None
+        if not any(t is not None and t.requires_grad for t in (x, f, gate)):
+            anchor = torch.empty(0, device=x.device, requires_grad=True)
+        out = _ResNormFn.apply(x, f, gate if gate is None else gate.contiguous(), anchor, self)
         return (x, out) if f is None else out if self.pre is not None else (out, None)

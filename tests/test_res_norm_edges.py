@@ -186,3 +186,31 @@ def test_gradients_without_their_input_are_refused():
         e = lib.ResNormDesc.from_buffer_copy(d)
         setattr(e, name, 16)
         assert lib.call_raw('mscl_res_norm_bwd', ctypes.byref(e), None) == -1, name
+
+
+@pytest.mark.gpu
+def test_captured_beside_a_living_eager_graph(dev):
+    """a forward and backward pass captured while the graph of an eager pass over the same module lives; three replays against eager passes"""
+    m, ar = _module(dev)
+    x, f, dy = torch.randn(12, 16, device=dev), torch.randn(12, 16, device=dev), torch.randn(12, 16, device=dev)
+    keep, _ = m(x.clone(), f.clone())         # never differentiated before the capture; no input needs a gradient
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ar.G.zero_()
+        y, _ = m(x, f)
+        torch.autograd.backward([y], [dy])
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        got, out = ar.G.clone(), y.detach().clone()
+        ar.G.zero_()
+        y2, _ = m(x, f)
+        torch.autograd.backward([y2], [dy])
+        torch.cuda.synchronize()
+        assert torch.equal(got, ar.G) and torch.equal(out, y2) and got.any()
+        x.mul_(0.7)
+        dy.add_(0.1)
+    first = ar.G.clone()
+    torch.autograd.backward([keep], [torch.zeros_like(dy)])          # the eager graph is still whole
+    assert torch.equal(first, ar.G)
