@@ -23,6 +23,7 @@
 // 16384 x 4096, fp32 / bf16, a gate per element: 1.48 GB in 304 us, 4.9 TB/s.  The second launch of a backward pass: 6 - 20 us.
 #include "common.h"
 #include <hip/hip_fp16.h>
+#include <atomic>
 
 namespace {
 __device__ __forceinline__ float h2f(uint16_t h) { return __half2float(__ushort_as_half(h)); }
@@ -683,48 +684,51 @@ void res_norm_fwd_types(const mscl_res_norm_desc& d, hipStream_t st) {
   else fwd_launch<XT, FT, 2, false>(d, T, (unsigned)grid, share, st);
 }
 template <int XT, int FT, int NV, bool WAVE, int THREADS, int MODE, bool BIAS, bool NARROW = false>
-static void bwd_go(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
+static int bwd_go(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
   constexpr int IN_LDS = bwd_in_lds(NV, THREADS, XT, MODE, BIAS);
   const int bytes = WAVE ? 256 * 8 * NV * 4 : IN_LDS / (BIAS ? 1 : 2) * NV * 32 * p.T;
   if constexpr (IN_LDS) {
-    static uint64_t told = 0;                         // a bit per device
+    static std::atomic<uint64_t> told{0};             // a bit for each of the first 64 devices
     int dev = 0;
-    (void)hipGetDevice(&dev);
-    if (!(told >> (dev & 63) & 1)) {
-      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
-      told |= (uint64_t)1 << (dev & 63);
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return (int)e;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (!(told.load(std::memory_order_relaxed) & bit)) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
+      if (e != hipSuccess) return (int)e;
+      told.fetch_or(bit, std::memory_order_relaxed);
     }
   }
   hipLaunchKernelGGL((res_norm_bwd_kernel<XT, FT, NV, WAVE, THREADS, MODE, BIAS, NARROW>), dim3(p.blocks), dim3(WAVE ? 256 : p.T), bytes, st, d, p);
+  MSCL_LAUNCH_CHECK();
+  return 0;
 }
 template <int XT, int FT, int NV, bool WAVE, int THREADS>
-static void bwd_launch(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
+static int bwd_launch(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
   // the rare forms (rows below 8 channels, short runs per gate) carry the bias sums always
   if constexpr (WAVE) {
     if (d.C < 8) {
-      if (p.mode == WHOLE) bwd_go<XT, FT, NV, WAVE, THREADS, WHOLE, true, true>(d, p, st);
-      else if (p.mode == SPLIT) bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, true, true>(d, p, st);
-      else bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, true, true>(d, p, st);
-      return;
+      if (p.mode == WHOLE) return bwd_go<XT, FT, NV, WAVE, THREADS, WHOLE, true, true>(d, p, st);
+      if (p.mode == SPLIT) return bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, true, true>(d, p, st);
+      return bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, true, true>(d, p, st);
     }
   }
   if (p.mode == WHOLE) return bwd_go<XT, FT, NV, WAVE, THREADS, WHOLE, true>(d, p, st);
   if (d.b_post || d.b_pre) {
-    if (p.mode == SPLIT) bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, true>(d, p, st);
-    else bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, true>(d, p, st);
-  } else {
-    if (p.mode == SPLIT) bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, false>(d, p, st);
-    else bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, false>(d, p, st);
+    if (p.mode == SPLIT) return bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, true>(d, p, st);
+    return bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, true>(d, p, st);
   }
+  if (p.mode == SPLIT) return bwd_go<XT, FT, NV, WAVE, THREADS, SPLIT, false>(d, p, st);
+  return bwd_go<XT, FT, NV, WAVE, THREADS, EACH1, false>(d, p, st);
 }
 template <int XT, int FT>
 int res_norm_bwd_types(const mscl_res_norm_desc& d, const BwdPlan& p, hipStream_t st) {
-  if (p.wave) bwd_launch<XT, FT, 1, true, 256>(d, p, st);
-  else if (p.nv == 2) bwd_launch<XT, FT, 2, false, 1024>(d, p, st);
-  else if (p.T <= 512) bwd_launch<XT, FT, 1, false, 512>(d, p, st);
-  else if (p.T <= 768) bwd_launch<XT, FT, 1, false, 768>(d, p, st);        // 168 registers a lane; 1024 lanes leave 128
-  else bwd_launch<XT, FT, 1, false, 1024>(d, p, st);
-  MSCL_LAUNCH_CHECK();
+  const int rc = p.wave ? bwd_launch<XT, FT, 1, true, 256>(d, p, st)
+               : p.nv == 2 ? bwd_launch<XT, FT, 2, false, 1024>(d, p, st)
+               : p.T <= 512 ? bwd_launch<XT, FT, 1, false, 512>(d, p, st)
+               : p.T <= 768 ? bwd_launch<XT, FT, 1, false, 768>(d, p, st)        // 168 registers a lane; 1024 lanes leave 128
+               : bwd_launch<XT, FT, 1, false, 1024>(d, p, st);
+  if (rc) return rc;
   // few columns a block for narrow rows (few blocks), whole 64-byte segments for wide ones (C = 64 / 1024, 3 M elements, a training pass: 36 / 49 us
   // with 4 columns, 38 / 38 with 16; this launch at C = 1000 / 768 / 568: 29 / 18 / 19 us with 4, 17 / 13 / 13 with 8, 18 / 13 / 17 with 16)
   const int cols = d.C < 512 ? 4 : d.C < 1024 ? 8 : 16;

@@ -86,3 +86,42 @@ def test_wide_odd_rows_captured(C, dev):
         torch.cuda.synchronize()
         assert torch.equal(y, y2) and torch.equal(h, h2) and all(torch.equal(v, g2[k]) for k, v in g.items())
         t['x'].mul_(0.7)
+
+
+def test_wide_backward_without_a_device():
+    """the entry point reports what the runtime says to it before the launch, too (here: that there is no GPU), instead of launching on"""
+    import ctypes
+
+    from mscl_amd import lib
+    if torch.cuda.is_available():
+        pytest.skip('needs a host without a GPU')
+    d = lib.ResNormDesc(x=16, f=16, dy=16, dh=16, rstd_f=16, rstd_y=16, ws=16, rows=4, C=8192, ld_x=8192, ld_f=8192, x_type=2, f_type=2, post=1, pre=1,
+                        eps=1e-6)
+    d.ws_floats = lib.call_raw('mscl_res_norm_ws', ctypes.byref(d))
+    assert lib.call_raw('mscl_res_norm_bwd', ctypes.byref(d), None) > 0
+
+
+@pytest.mark.gpu
+def test_wide_backward_from_several_threads(dev):
+    """calls from four threads at once, a stream each, the first calls of these forms in the process or not: the results of one thread"""
+    import threading
+
+    from mscl_amd import kernels as K_
+    C = 8000
+    t = _inputs(8, C, 8, F, H, dev, 1)
+    _, _, saved = K_.res_norm_fwd(t['x'], t['f'], gate=t['gate'], post_norm='rms', pre_norm='layer', save=True, **{k: t[k] for k in VECS})
+    torch.cuda.synchronize()
+    got, streams = [None] * 4, [torch.cuda.Stream() for _ in range(4)]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            got[i] = K_.res_norm_bwd(saved, t['dy'], t['dh'])
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    want = K_.res_norm_bwd(saved, t['dy'], t['dh'])
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, g[k]) for g in got for k, v in want.items())
