@@ -345,6 +345,7 @@ static int adamw_launch(const mscl_adamw_desc& d, hipStream_t st) {
 extern "C" int mscl_adamw_step(const mscl_adamw_desc* d, void* stream) {
   if (!d || !d->tensors || !d->grads || !d->chunk_tensor || !d->m || !d->v || !d->words || !d->lr || d->n_chunks <= 0) return MSCL_E_ARG;
   if (!(d->beta1 >= 0 && d->beta1 < 1 && d->beta2 >= 0 && d->beta2 < 1 && d->eps > 0)) return MSCL_E_ARG;
+  if (!(d->max_norm > 0 || d->max_norm <= 0)) return MSCL_E_ARG;          // NaN
   if (d->max_norm > 0 && (!d->partials || !d->grad_norm)) return MSCL_E_ARG;
   if (d->state_bits != 32 && d->state_bits != 8) return MSCL_E_SHAPE;
   if (d->state_bits == 8 && (!d->exponents || d->n_blocks <= 0)) return MSCL_E_ARG;

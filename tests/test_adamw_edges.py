@@ -1,0 +1,21 @@
+"""Calls of the AdamW step at the ends of their range, its checkpoints across other parameters and other optimizers, and what autograd sees of
+it."""
+import ctypes
+import os
+import re
+
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+U = 2.0 ** -24
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_a_clip_that_is_no_number_is_refused_by_the_library():
+    """without a clip `partials` and `grad_norm` may be NULL, so a max_norm that compares neither way must not get to the kernels"""
+    from mscl_amd import lib
+    d = lib.AdamWDesc(tensors=16, grads=16, chunk_tensor=16, m=16, v=16, words=16, lr=16, beta1=0.9, beta2=0.999, eps=1e-8, max_norm=float('nan'),
+                      n_chunks=1, state_bits=32, grad_type=1)
+    assert lib.call_raw('mscl_adamw_step', ctypes.byref(d), None) == -1
