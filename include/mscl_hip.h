@@ -412,7 +412,7 @@ int mscl_cast_bf16(const float* src, uint16_t* dst, int64_t n, void* stream);
  *   step t = ++words.step;  c = min(1, max_norm / (|g| + 1e-6)) (1 when max_norm <= 0), *grad_norm = |g| before the clip;
  *   m = b1 m + (1-b1) c g;  v = b2 v + (1-b2) (c g)^2;
  *   p = p (1 - lr lr_mult decay) - lr lr_mult / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps);  shadow = round(p)
- * Bit-reproducible (no atomics).  A non-finite gradient behaves as in torch: it goes into m, v and p.
+ * eps >= 2^-126.  Bit-reproducible (no atomics).  A non-finite gradient behaves as in torch: it goes into m, v and p.
  * States: flat buffers in which tensor i starts at element `off`, a multiple of MSCL_ADAMW_BLOCK, and is padded with zeros to a whole
  * number of blocks.  8 bits: one byte per element and moment plus, per block and moment, one exponent byte E (fp32's bias; 255: the
  * block holds a non-finite value and reads as NaN).  m: sign, 4-bit exponent field e, 3-bit mantissa k, value (1 + k/8) 2^(E-127 + e-15)

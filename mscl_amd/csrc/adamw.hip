@@ -20,6 +20,7 @@
 // about four fifths of the time (78 instructions per element, two of them quarter-rate multiplies of the hash).
 #include "common.h"
 #include <hip/hip_fp16.h>
+#include <cfloat>
 
 namespace {
 constexpr int CHUNK = 4096;          // elements a block of 256 threads takes: 4 vectors of 4 per thread and array, 16 loads in flight (32 bits)
@@ -344,7 +345,8 @@ static int adamw_launch(const mscl_adamw_desc& d, hipStream_t st) {
 }
 extern "C" int mscl_adamw_step(const mscl_adamw_desc* d, void* stream) {
   if (!d || !d->tensors || !d->grads || !d->chunk_tensor || !d->m || !d->v || !d->words || !d->lr || d->n_chunks <= 0) return MSCL_E_ARG;
-  if (!(d->beta1 >= 0 && d->beta1 < 1 && d->beta2 >= 0 && d->beta2 < 1 && d->eps > 0)) return MSCL_E_ARG;
+  if (!(d->beta1 >= 0 && d->beta1 < 1 && d->beta2 >= 0 && d->beta2 < 1)) return MSCL_E_ARG;
+  if (!((float)d->eps >= FLT_MIN)) return MSCL_E_ARG;          // the reciprocal of a subnormal is infinite
   if (!(d->max_norm > 0 || d->max_norm <= 0)) return MSCL_E_ARG;          // NaN
   if (d->max_norm > 0 && (!d->partials || !d->grad_norm)) return MSCL_E_ARG;
   if (d->state_bits != 32 && d->state_bits != 8) return MSCL_E_SHAPE;

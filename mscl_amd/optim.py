@@ -184,8 +184,8 @@ def _check_grad_memory(ptrs, nbytes, spans):
 def _check_args(lr, betas, eps, weight_decay, grad_clip, state_bits, seed=0):
     if state_bits not in (32, 8):
         raise MsclError(f'AdamW: state_bits is 32 or 8, not {state_bits}')
-    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and np.float32(eps) > 0 and lr >= 0 and weight_decay >= 0):
-        raise MsclError('AdamW: needs 0 <= betas < 1, eps > 0 in fp32, lr >= 0, weight_decay >= 0')
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and np.float32(eps) >= np.finfo(np.float32).tiny and lr >= 0 and weight_decay >= 0):
+        raise MsclError('AdamW: needs 0 <= betas < 1, eps of at least 2^-126 (the least normal fp32 number), lr >= 0, weight_decay >= 0')
     if grad_clip is not None and grad_clip.get('norm_type', 2) != 2:
         raise NotImplementedError('only the L2 norm is used (optimizer_config.grad_clip.norm_type=2)')
     if grad_clip is not None and not grad_clip['max_norm'] > 0:

@@ -19,3 +19,17 @@ def test_a_clip_that_is_no_number_is_refused_by_the_library():
     d = lib.AdamWDesc(tensors=16, grads=16, chunk_tensor=16, m=16, v=16, words=16, lr=16, beta1=0.9, beta2=0.999, eps=1e-8, max_norm=float('nan'),
                       n_chunks=1, state_bits=32, grad_type=1)
     assert lib.call_raw('mscl_adamw_step', ctypes.byref(d), None) == -1
+
+
+def test_eps_below_the_normal_range_is_refused():
+    """the reciprocal of a subnormal is infinite, and an element with no gradient yet would be 0 * inf"""
+    from mscl_amd import lib, optim
+    from mscl_amd.lib import MsclError
+    for eps in (1e-38, 1e-45):
+        with pytest.raises(MsclError, match='eps'):
+            optim.AdamW([torch.zeros(3)], eps=eps)
+    with pytest.raises(MsclError, match='no CPU fallback'):
+        optim.AdamW([torch.zeros(3)], eps=1.2e-38)
+    d = lib.AdamWDesc(tensors=16, grads=16, chunk_tensor=16, m=16, v=16, words=16, lr=16, beta1=0.9, beta2=0.999, eps=1e-38, n_chunks=1,
+                      state_bits=32, grad_type=1)
+    assert lib.call_raw('mscl_adamw_step', ctypes.byref(d), None) == -1
