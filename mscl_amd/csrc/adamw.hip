@@ -191,6 +191,25 @@ __global__ __launch_bounds__(256) void adamw_coef_kernel(mscl_adamw_desc d, int 
   if (threadIdx.x == 0) ((Words*)d.words)->coef = clip_coef(d, red, true);
 }
 
+// sqrt of four second moments by the 1-ulp instruction, which takes a subnormal for 0: where a wave has one (gradients below 1e-18, where a
+// small eps is all that is left in the denominator), those go through it 2^64 times as large.  One class test an element otherwise.
+__device__ __forceinline__ void sqrt4(const float* v, float* r) {
+  bool sub = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = __builtin_amdgcn_sqrtf(v[i]);
+    sub |= __builtin_amdgcn_classf(v[i], 0x080);                  // positive subnormal
+  }
+  if (__builtin_amdgcn_ballot_w64(sub)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool low = v[i] < FLT_MIN;
+      const float s = __builtin_amdgcn_sqrtf(low ? v[i] * 0x1p64f : v[i]);
+      r[i] = low ? s * 0x1p-32f : s;
+    }
+  }
+}
+
 // A block owns CHUNK elements of one tensor; the loads of all four vectors of a thread go out before the first is used.
 template <int GT, int ST, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(mscl_adamw_desc d, int parts) {
@@ -268,7 +287,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(mscl_adamw_desc d, int parts
       const float gi = gv[k][i] * coef;
       m[i] = m[i] * b1 + gi * a1;
       v[i] = v[i] * b2 + gi * gi * a2;
-      const float den = __builtin_amdgcn_sqrtf(v[i]) * c2 + eps;
+    }
+    float root[4];
+    sqrt4(v, root);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float den = root[i] * c2 + eps;
       pv[k][i] = pv[k][i] * keep - rate * m[i] * __builtin_amdgcn_rcpf(den);
     }
     if (whole || e + 4 <= n) {

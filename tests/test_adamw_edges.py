@@ -33,3 +33,23 @@ def test_eps_below_the_normal_range_is_refused():
     d = lib.AdamWDesc(tensors=16, grads=16, chunk_tensor=16, m=16, v=16, words=16, lr=16, beta1=0.9, beta2=0.999, eps=1e-38, n_chunks=1,
                       state_bits=32, grad_type=1)
     assert lib.call_raw('mscl_adamw_step', ctypes.byref(d), None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('eps', [1e-8, 1e-15, 1e-20, 1e-30, 2e-38])
+def test_second_moments_below_the_normal_range(eps, bits, dev):
+    """gradients whose squares are subnormal, beside zeros and ordinary ones: the first step against the formula on the second moment as fp32
+    holds it.  24 u of the update and 4 u of p (as derived in test_adamw.py), whatever eps is."""
+    from mscl_amd import AdamW
+    g = torch.cat([torch.zeros(5)] + [torch.full((7,), 10.0 ** -k) * (1 + torch.arange(7) / 7) for k in (2, 8, 14, 17, 18, 19, 20, 21)])
+    p = torch.zeros(g.numel(), device=dev)
+    opt = AdamW([p], lr=1.0, eps=eps, weight_decay=0.0, state_bits=bits)
+    opt.step([g.to(dev)])
+    G = g.numpy()
+    v = (G * G) * np.float32(1 - 0.999)
+    assert v.dtype == np.float32 and ((v > 0) & (v < 2.0 ** -126)).sum() > 10
+    m = G.astype(np.float64) * 0.1
+    want = -(m / (1 - 0.9)) / (np.sqrt(v.astype(np.float64) / (1 - 0.999)) + float(np.float32(eps)))
+    got = p.cpu().double().numpy()
+    assert (np.abs(got - want) <= 28 * U * np.abs(want) + 1e-38).all(), (got / np.where(want == 0, 1, want)).tolist()
