@@ -21,12 +21,15 @@
 #include "common.h"
 #include <hip/hip_fp16.h>
 #include <cfloat>
+#include <cstddef>
 
 namespace {
-constexpr int CHUNK = 4096;          // elements a block of 256 threads takes: 4 vectors of 4 per thread and array, 16 loads in flight (32 bits)
+constexpr int CHUNK = MSCL_ADAMW_CHUNK;        // elements a block of 256 threads takes: 4 vectors of 4 per thread and array, 16 loads in flight (32 bits)
 constexpr int PARTS = MSCL_ADAMW_PARTS;
+static_assert(CHUNK == 256 * 4 * 4 && MSCL_ADAMW_BLOCK == 64 * 4, "the kernels' shape");
 
 struct Words { int64_t step; float c1, c2; uint32_t key, seed; float coef; uint32_t pad; };      // = the words buffer
+static_assert(sizeof(Words) == MSCL_ADAMW_WORDS && offsetof(Words, seed) == 20, "the words buffer");
 
 // The update passes once over far more memory than any cache holds: its accesses are marked non-temporal, which leaves the caches to the
 // gradient between the launches (33 M elements, fp32 / clip / shadow: a step of 238 -> 200 us; 320 M without clip: 1611 -> 1507 us).

@@ -53,3 +53,11 @@ def test_second_moments_below_the_normal_range(eps, bits, dev):
     want = -(m / (1 - 0.9)) / (np.sqrt(v.astype(np.float64) / (1 - 0.999)) + float(np.float32(eps)))
     got = p.cpu().double().numpy()
     assert (np.abs(got - want) <= 28 * U * np.abs(want) + 1e-38).all(), (got / np.where(want == 0, 1, want)).tolist()
+
+
+def test_kernel_constants_are_the_headers():
+    """chunk, block, number of partial sums and the layout of the words buffer are written once, in the header"""
+    src = open(os.path.join(ROOT, 'mscl_amd', 'csrc', 'adamw.hip')).read()
+    for name in ('CHUNK', 'PARTS'):
+        assert re.search(rf'constexpr int {name} = MSCL_ADAMW_{name};', src), name
+    assert 'sizeof(Words) == MSCL_ADAMW_WORDS' in src and 'MSCL_ADAMW_BLOCK ==' in src
