@@ -257,6 +257,7 @@ class AdamW:
             self._lr_sent = float(lr)
             self._grad_ring = StagingRing((n,), torch.int64, self.device)
         self._grad_ptrs, self._in_graph, self._kept = None, False, []
+        self._written = [t for t in self._leaves + (self.shadows or []) if not t.is_inference()]
         P = lib.ptr
         self._desc = AdamWDesc(P(self._table), P(self._grad_ring.dev), P(self._chunk_tensor), P(self.exp_avg), P(self.exp_avg_sq),
                                P(self.exponents), total // BLOCK, P(self._words), P(self._partials), P(self._norm), P(self._lr.dev),
@@ -302,6 +303,7 @@ class AdamW:
                 return self.step(grads)
         self._set_grads(grads)
         self._launch()
+        torch.autograd.graph.increment_version(self._written)          # a backward pass over a graph from before the step is refused
 
     def _launch(self):
         capturing = torch.cuda.is_current_stream_capturing()

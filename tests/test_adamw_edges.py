@@ -61,3 +61,33 @@ def test_kernel_constants_are_the_headers():
     for name in ('CHUNK', 'PARTS'):
         assert re.search(rf'constexpr int {name} = MSCL_ADAMW_{name};', src), name
     assert 'sizeof(Words) == MSCL_ADAMW_WORDS' in src and 'MSCL_ADAMW_BLOCK ==' in src
+
+
+@pytest.mark.gpu
+def test_a_step_invalidates_graphs_of_before(dev):
+    """a backward pass over a graph from before the step would use the new weights in the place of the saved ones: refused, as after any
+    other in-place change; shadows count too"""
+    from mscl_amd import AdamW
+    net = nn.Sequential(nn.Linear(8, 8), nn.Linear(8, 3)).to(dev)
+    opt = AdamW(net.parameters(), lr=1e-2)
+    x = torch.randn(4, 8, device=dev)
+    loss = net(x).square().sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    opt.zero_grad()
+    net(x).square().sum().backward()
+    opt.step()
+    master = torch.randn(8, 8, device=dev)
+    shadow = master.bfloat16().requires_grad_()
+    opt = AdamW([master], shadows=[shadow.detach()])
+    x16 = x.bfloat16().requires_grad_()
+    out = (x16 @ shadow).float().sum()
+    opt.step([torch.ones(8, 8, device=dev)])
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        out.backward()
+    with torch.inference_mode():
+        p = torch.zeros(5, device=dev)
+    AdamW([p]).step([torch.ones(5, device=dev)])          # (a tensor without a version counter is stepped as before)
+    assert bool((p < 0).all())
