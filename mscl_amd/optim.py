@@ -192,6 +192,9 @@ def _check_args(lr, betas, eps, weight_decay, grad_clip, state_bits, seed=0):
         raise MsclError('AdamW: grad_clip needs max_norm > 0 (None: no clip)')
 
 
+_raise_version = getattr(torch._C, '_increment_version', None) or torch.autograd.graph.increment_version          # (raw: 4 / 62 tensors 0.6 / 4.0 us, not 1.2 / 5.6)
+
+
 class AdamW:
     """AdamW with decoupled decay over a list of fp32 GPU tensors, two or three launches per step whatever their number.
 
@@ -303,7 +306,7 @@ class AdamW:
                 return self.step(grads)
         self._set_grads(grads)
         self._launch()
-        torch.autograd.graph.increment_version(self._written)          # a backward pass over a graph from before the step is refused
+        _raise_version(self._written)          # a backward pass over a graph from before the step is refused
 
     def _launch(self):
         capturing = torch.cuda.is_current_stream_capturing()
