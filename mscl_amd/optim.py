@@ -308,9 +308,16 @@ class AdamW:
         self._launch()
         _raise_version(self._written)          # a backward pass over a graph from before the step is refused
 
+    def _check_groups(self):
+        g = self.param_groups[0]
+        if (len(self.param_groups) > 1 or g.get('weight_decay', self.wd) != self.wd or g.get('eps', self.eps) != self.eps
+                or tuple(g.get('betas', self.betas)) != self.betas):
+            raise MsclError('AdamW: betas, eps and weight_decay are fixed when the optimizer is built, of param_groups[0] lr alone is read')
+
     def _launch(self):
         capturing = torch.cuda.is_current_stream_capturing()
         if capturing:
+            self._check_groups()
             self._in_graph = True
         else:                                               # a captured step publishes before each replay
             self.sync_lr()
@@ -319,6 +326,7 @@ class AdamW:
 
     def sync_lr(self):
         """publish param_groups[0]['lr'] to the device word the kernel reads, in stream order.  Unchanged values are not re-sent."""
+        self._check_groups()
         lr = float(self.param_groups[0]['lr'])
         if lr == self._lr_sent:
             return

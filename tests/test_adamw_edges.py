@@ -91,3 +91,25 @@ def test_a_step_invalidates_graphs_of_before(dev):
         p = torch.zeros(5, device=dev)
     AdamW([p]).step([torch.ones(5, device=dev)])          # (a tensor without a version counter is stepped as before)
     assert bool((p < 0).all())
+
+
+@pytest.mark.gpu
+def test_changed_settings_are_refused(dev):
+    """lr is read at every step; a change of the others would be ignored"""
+    from mscl_amd import AdamW
+    from mscl_amd.lib import MsclError
+    p, g = torch.zeros(5, device=dev), torch.ones(5, device=dev)
+    opt = AdamW([p], lr=1e-2)
+    opt.step([g])
+    for key, v in (('weight_decay', 0.5), ('eps', 1e-3), ('betas', (0.5, 0.9))):
+        old = opt.param_groups[0][key]
+        opt.param_groups[0][key] = v
+        before = p.clone()
+        with pytest.raises(MsclError, match='param_groups'):
+            opt.step([g])
+        with pytest.raises(MsclError, match='param_groups'):
+            opt.sync_lr()
+        assert torch.equal(p, before) and opt.device_step() == 1
+        opt.param_groups[0][key] = list(old) if key == 'betas' else old
+    opt.step([g])
+    assert opt.device_step() == 2
