@@ -287,18 +287,20 @@ class AdamW:
             alike = False
         if not alike:   # one by one: names what does not fit, or finds that it does
             _check_grads(grads, self.params)
-        ptrs = list(map(T.data_ptr, grads))
-        if ptrs != self._grad_ptrs:
-            if torch.cuda.is_current_stream_capturing():
-                raise MsclError('AdamW: a step is captured with the gradient tensors of the eager step before it (a capture cannot upload other addresses)')
+        ptrs, kind = list(map(T.data_ptr, grads)), _TYPES[grads[0].dtype]
+        moved = ptrs != self._grad_ptrs
+        if moved and torch.cuda.is_current_stream_capturing():
+            raise MsclError('AdamW: a step is captured with the gradient tensors of the eager step before it (a capture cannot upload other addresses)')
+        if moved or kind != self._desc.grad_type:
             _check_grad_memory(ptrs, [g.numel() * g.element_size() for g in grads], self._spans)
+        if moved:
             if self._in_graph:                  # a captured step reads the old table: leave it as it is, with its gradients' addresses
                 self._kept.append(self._grad_ring)
                 self._grad_ring, self._in_graph = StagingRing((len(ptrs),), torch.int64, self.device), False
                 self._desc.grads = lib.ptr(self._grad_ring.dev)
             self._grad_ring.push(torch.tensor(ptrs, dtype=torch.int64))
             self._grad_ptrs = ptrs
-        self._desc.grad_type = _TYPES[grads[0].dtype]
+        self._desc.grad_type = kind
 
     def step(self, grads=None):
         if torch.cuda.current_device() != self.device.index:

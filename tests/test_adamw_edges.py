@@ -113,3 +113,19 @@ def test_changed_settings_are_refused(dev):
         opt.param_groups[0][key] = list(old) if key == 'betas' else old
     opt.step([g])
     assert opt.device_step() == 2
+
+
+@pytest.mark.gpu
+def test_gradients_of_another_type_at_the_same_address(dev):
+    """wider gradients at the address of narrow ones reach further: their memory is looked at again"""
+    from mscl_amd import AdamW
+    from mscl_amd.lib import MsclError
+    buf = torch.zeros(64, device=dev)
+    p = buf[16:48]                                         # bytes 64 .. 191
+    g16 = buf.view(torch.bfloat16)[:32]                    # bytes 0 .. 63
+    opt = AdamW([p])
+    opt.step([g16])
+    with pytest.raises(MsclError, match='share memory'):
+        opt.step([buf[:32]])                               # bytes 0 .. 127
+    opt.step([g16])
+    assert opt.device_step() == 2
