@@ -235,7 +235,7 @@ class AdamW:
         off, first, total, n_chunks, chunks = _layout(sizes)
         if n_chunks >= 1 << 31:
             raise MsclError('AdamW: too many elements for one step')
-        self.offsets, self.numel = off.tolist(), total
+        self.sizes, self.offsets, self.numel = sizes, off.tolist(), total
         with torch.cuda.device(self.device):
             table = np.zeros(n, dtype=_TENSOR)
             table['p'] = [p.data_ptr() for p in self.params]
@@ -360,8 +360,8 @@ class AdamW:
         self.steps = int(step)
 
     def state_dict(self):
-        """flat states (tensor i at self.offsets[i]), on the device; synchronises for the step counter"""
-        out = dict(step=self.device_step(), state_bits=self.state_bits, lr=self.param_groups[0]['lr'], seed=self.seed,
+        """flat states (tensor i at self.offsets[i], sizes[i] elements), on the device; synchronises for the step counter"""
+        out = dict(step=self.device_step(), state_bits=self.state_bits, lr=self.param_groups[0]['lr'], seed=self.seed, sizes=list(self.sizes),
                    exp_avg=self.exp_avg.clone(), exp_avg_sq=self.exp_avg_sq.clone())
         if self.state_bits == 8:
             out['exponents'] = self.exponents.clone()
@@ -372,6 +372,8 @@ class AdamW:
             raise MsclError(f"AdamW: a state of {state['state_bits']} bits does not fit state_bits={self.state_bits}")
         if state['step'] < 0:
             raise MsclError('AdamW: a negative step')
+        if list(state.get('sizes', self.sizes)) != self.sizes:          # (states written without them are told by the total alone)
+            raise MsclError('AdamW: the state belongs to other parameters')
         pairs = [(self.exp_avg, state['exp_avg']), (self.exp_avg_sq, state['exp_avg_sq'])]
         if self.state_bits == 8:
             pairs.append((self.exponents, state['exponents']))

@@ -129,3 +129,31 @@ def test_gradients_of_another_type_at_the_same_address(dev):
         opt.step([buf[:32]])                               # bytes 0 .. 127
     opt.step([g16])
     assert opt.device_step() == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+def test_states_of_other_tensors_are_refused(bits, dev):
+    """the flat states belong to a list of tensors: another list that pads to as many blocks does not take them"""
+    from mscl_amd import AdamW
+    from mscl_amd.lib import MsclError
+
+    def make(sizes):
+        ps = [torch.zeros(n, device=dev) for n in sizes]
+        opt = AdamW(ps, state_bits=bits)
+        opt.step([torch.ones_like(p) for p in ps])
+        return opt
+    a = make([300, 10, 77])
+    state = a.state_dict()
+    for sizes in ([10, 300, 77], [300, 77, 10], [300, 256, 256], [768, 256]):
+        b = make(sizes)
+        assert b.numel == a.numel
+        before = b.state_dict()
+        with pytest.raises(MsclError, match='other parameters'):
+            b.load_state_dict(state)
+        after = b.state_dict()
+        assert all(torch.equal(v, after[k]) if torch.is_tensor(v) else v == after[k] for k, v in before.items())
+    c = make([300, 10, 77])
+    c.load_state_dict(state)
+    old = {k: v for k, v in state.items() if k in ('step', 'state_bits', 'lr', 'seed', 'exp_avg', 'exp_avg_sq', 'exponents')}
+    c.load_state_dict(old)                                 # a state written without the sizes
