@@ -413,6 +413,19 @@ def _param_mults(named_params, norm_params, cfg):
     return lr_mult, decay_mult
 
 
+def _base_lr(groups, mult):
+    """the rate that every one of torch's parameter groups gives for a parameter of multiplier 1 (mmcv's constructor writes a group for each
+    parameter, lr times its multiplier); None where no group tells.  mult: lr multiplier of each parameter index"""
+    if any(not 0 <= i < len(mult) for g in groups for i in g.get('params', ())):
+        raise MsclError("ClipAdamW: the state's groups hold parameters that the model has not")
+    rates = [float(g['lr']) / mult[i] for g in groups if 'lr' in g for i in g.get('params', ()) if mult[i] > 0]
+    if not rates:
+        return float(groups[0]['lr']) if 'lr' in groups[0] and 'params' not in groups[0] else None
+    if max(rates) - min(rates) > 1e-6 * max(rates):
+        raise MsclError(f'ClipAdamW: the state holds rates from {min(rates)} to {max(rates)} without their lr_mult: built with another paramwise_cfg')
+    return rates[0]
+
+
 class ClipAdamW:
     """Clip + AdamW over a model's arena: what ClipSGD is, with `AdamW` in place of the SGD pass.  The parameters that have received a
     gradient by the first step take part (those that never do are left alone, as torch leaves a parameter without .grad)."""
@@ -510,26 +523,29 @@ class ClipAdamW:
             return
         if self.state_bits != 32:
             raise MsclError('ClipAdamW: a torch.optim.AdamW state loads into state_bits=32')
-        found, step = [], 0
-        for idx, p in enumerate(self.model.parameters()):
+        found, step, params = [], 0, list(self.model.parameters())
+        for idx, p in enumerate(params):
             st = state['state'].get(idx, state['state'].get(str(idx)))
             if st is None:
                 continue
             slot = getattr(p, '_mscl_slot', None)
             if slot is None or not p.requires_grad or tuple(st['exp_avg'].shape) != tuple(p.shape):
                 raise ValueError(f'optimizer state {idx} does not belong to trainable parameter {idx} of this model')
-            slot.touched, step = True, max(step, int(st['step']))
+            step = max(step, int(st['step']))
             found.append((slot, st))
         if not found:
             raise MsclError('ClipAdamW: the checkpoint holds no AdamW moments')
+        mult = [self._mult.get(getattr(p, '_mscl_slot', None), (1.0, 1.0))[0] if p.requires_grad else 1.0 for p in params]
+        lr = _base_lr(state.get('param_groups') or [{}], mult)
+        for slot, _ in found:
+            slot.touched = True
         self._build()
         at = dict(zip(self._slots, self._inner.offsets))
         for slot, st in found:
             for flat, key in ((self._inner.exp_avg, 'exp_avg'), (self._inner.exp_avg_sq, 'exp_avg_sq')):
                 _physical_view(flat, at[slot], slot.shape).copy_(st[key])
-        groups = state.get('param_groups') or [{}]
-        if 'lr' in groups[0]:
-            self.param_groups[0]['lr'] = groups[0]['lr']
+        if lr is not None:
+            self.param_groups[0]['lr'] = lr
         self._inner.set_step(step)
         self.steps = step
 

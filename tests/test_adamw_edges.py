@@ -157,3 +157,88 @@ def test_states_of_other_tensors_are_refused(bits, dev):
     c.load_state_dict(state)
     old = {k: v for k, v in state.items() if k in ('step', 'state_bits', 'lr', 'seed', 'exp_avg', 'exp_avg_sq', 'exponents')}
     c.load_state_dict(old)                                 # a state written without the sizes
+
+
+class _Net(nn.Module):
+    """three norms bound to an arena; `first` and `last` may have rates of their own"""
+
+    def __init__(self):
+        super().__init__()
+        from mscl_amd.nn import ResNormHip
+        self.first, self.mid, self.last = ResNormHip(24, None, 'rms'), ResNormHip(24, 'rms', None, scale=0.5), ResNormHip(24, 'layer', None, bias=True)
+
+    def forward(self, x, upto=3):
+        x, h = self.first(x)
+        if upto > 1:
+            x, _ = self.mid(x, h)
+        if upto > 2:
+            x, _ = self.last(x, h)
+        return x if upto > 1 else h
+
+    def sync_streams(self):
+        pass
+
+    def refresh_after_optimizer(self):
+        pass
+
+
+def _net(dev, bits=32, **cfg):
+    from mscl_amd import build_optimizer
+    from mscl_amd.arena import ParamArena
+    from mscl_amd.recognizers import bind_module
+    model, ar = _Net(), ParamArena(dev)
+    plan = [(ar.add(n, p.shape), p) for n, p in model.named_parameters()]
+    ar.allocate(with_key=False)
+    for slot, p in plan:
+        v = ar.view('Q', slot)
+        v.copy_(p.data)
+        p.data, p.grad, p._mscl_slot = v, ar.view('G', slot), slot
+    model.arena = ar
+    for m in model.modules():
+        bind_module(m, ar, False, model)
+    return model, build_optimizer(model, dict(type='AdamW', lr=1e-3, state_bits=bits, **cfg))
+
+
+def _train(model, opt, steps=1, upto=3):
+    for s in range(steps):
+        opt.zero_grad()
+        x = torch.randn(6, 24, generator=torch.Generator().manual_seed(s)).to(model.arena.device)
+        model(x, upto).square().sum().backward()
+        opt.step()
+
+
+def _torch_state(model, lrs, steps=1, skip=()):
+    """torch.optim.AdamW's state over the model's parameters, a group for each"""
+    ref = [p.detach().clone().requires_grad_() for p in model.parameters()]
+    groups = [dict(params=[p], lr=lr) for p, lr in zip(ref, lrs)]
+    opt = torch.optim.AdamW(groups)
+    for _ in range(steps):
+        for i, p in enumerate(ref):
+            p.grad = None if i in skip else torch.randn_like(p)
+        opt.step()
+    return opt.state_dict()
+
+
+@pytest.mark.gpu
+def test_paramwise_rates_of_a_torch_state(dev):
+    """torch's groups hold lr times the parameter's multiplier: the base rate is what is left without it, from whichever group; groups that
+    disagree, as under another paramwise_cfg, are refused and change nothing"""
+    from mscl_amd.lib import MsclError
+    from mscl_amd.optim import _param_mults
+    cfg = dict(custom_keys=dict(first=dict(lr_mult=0.1), last=dict(lr_mult=0.0)))
+    model, opt = _net(dev, paramwise_cfg=cfg)
+    mult, _ = _param_mults(list(model.named_parameters()), set(), cfg)
+    assert mult[0] == 0.1 and 1.0 in mult and mult[-1] == 0.0
+    opt.load_state_dict(_torch_state(model, [3e-4 * m for m in mult]))
+    assert abs(opt.param_groups[0]['lr'] / 3e-4 - 1) < 1e-12
+    one = _torch_state(model, [3e-4] * len(mult))
+    m2, o2 = _net(dev, paramwise_cfg=cfg)
+    with pytest.raises(MsclError, match='rate'):
+        o2.load_state_dict(one)
+    assert o2._inner is None and o2.param_groups[0]['lr'] == 1e-3 and not any(s.touched for s in m2.arena.slots)
+    m3, o3 = _net(dev)
+    o3.load_state_dict(one)
+    assert o3.param_groups[0]['lr'] == 3e-4
+    m4, o4 = _net(dev, paramwise_cfg=dict(norm_decay_mult=0.0, custom_keys=dict(first=dict(lr_mult=0.0), mid=dict(lr_mult=0.0), last=dict(lr_mult=0.0))))
+    o4.load_state_dict(_torch_state(m4, [0.0] * len(mult)))
+    assert o4.param_groups[0]['lr'] == 1e-3               # no group tells: as configured
