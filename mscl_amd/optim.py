@@ -541,6 +541,8 @@ class ClipAdamW:
             slot.touched = True
         self._build()
         at = dict(zip(self._slots, self._inner.offsets))
+        for flat in (self._inner.exp_avg, self._inner.exp_avg_sq):          # parameters without an entry have no moments
+            flat.zero_()
         for slot, st in found:
             for flat, key in ((self._inner.exp_avg, 'exp_avg'), (self._inner.exp_avg_sq, 'exp_avg_sq')):
                 _physical_view(flat, at[slot], slot.shape).copy_(st[key])

@@ -242,3 +242,20 @@ def test_paramwise_rates_of_a_torch_state(dev):
     m4, o4 = _net(dev, paramwise_cfg=dict(norm_decay_mult=0.0, custom_keys=dict(first=dict(lr_mult=0.0), mid=dict(lr_mult=0.0), last=dict(lr_mult=0.0))))
     o4.load_state_dict(_torch_state(m4, [0.0] * len(mult)))
     assert o4.param_groups[0]['lr'] == 1e-3               # no group tells: as configured
+
+
+@pytest.mark.gpu
+def test_moments_that_a_torch_state_lacks_start_at_zero(dev):
+    """loaded into an optimizer that has stepped: parameters without an entry have no moments, as in torch"""
+    model, opt = _net(dev)
+    _train(model, opt, 3)
+    n = len(list(model.parameters()))
+    state = _torch_state(model, [1e-3] * n, steps=2, skip=(1, n - 1))
+    opt.load_state_dict(state)
+    assert opt.steps == opt._inner.device_step() == 2
+    at = dict(zip(opt._slots, opt._inner.offsets))
+    for i, p in enumerate(model.parameters()):
+        for flat, key in ((opt._inner.exp_avg, 'exp_avg'), (opt._inner.exp_avg_sq, 'exp_avg_sq')):
+            got = flat[at[p._mscl_slot]:at[p._mscl_slot] + p.numel()].view(p.shape)
+            want = state['state'][i][key] if i in state['state'] else torch.zeros_like(p)
+            assert torch.equal(got, want.detach()), (i, key)
