@@ -523,6 +523,8 @@ class ClipAdamW:
             return
         if self.state_bits != 32:
             raise MsclError('ClipAdamW: a torch.optim.AdamW state loads into state_bits=32')
+        if any(g.get('amsgrad') for g in state.get('param_groups') or ()):
+            raise NotImplementedError('amsgrad is not built')
         found, step, params = [], 0, list(self.model.parameters())
         for idx, p in enumerate(params):
             st = state['state'].get(idx, state['state'].get(str(idx)))

@@ -259,3 +259,17 @@ def test_moments_that_a_torch_state_lacks_start_at_zero(dev):
             got = flat[at[p._mscl_slot]:at[p._mscl_slot] + p.numel()].view(p.shape)
             want = state['state'][i][key] if i in state['state'] else torch.zeros_like(p)
             assert torch.equal(got, want.detach()), (i, key)
+
+
+@pytest.mark.gpu
+def test_amsgrad_states_are_refused(dev):
+    """a maximum of second moments is no part of this step"""
+    model, opt = _net(dev)
+    ref = [p.detach().clone().requires_grad_() for p in model.parameters()]
+    topt = torch.optim.AdamW(ref, lr=1e-3, amsgrad=True)
+    for p in ref:
+        p.grad = torch.randn_like(p)
+    topt.step()
+    with pytest.raises(NotImplementedError, match='amsgrad'):
+        opt.load_state_dict(topt.state_dict())
+    assert opt._inner is None
