@@ -251,7 +251,7 @@ class AdamW:
             if state_bits == 8:        # 1: the smallest exponent, a block of zeros
                 self.exponents = torch.ones((2, total // BLOCK), dtype=torch.uint8, device=self.device)
             self._words = torch.zeros(WORDS // 4, dtype=torch.int32, device=self.device)
-            self._words[5] = ((self.seed & 0xFFFFFFFF) ^ 0x80000000) - 0x80000000          # 32 bits of the seed as an int32
+            self._set_seed(self.seed)
             self._partials = torch.zeros(PARTS, dtype=torch.float64, device=self.device)
             self._norm = torch.zeros(1, dtype=torch.float32, device=self.device)
             self._lr = StagingRing((1,), torch.float32, self.device)
@@ -359,6 +359,19 @@ class AdamW:
         self._words[:2].copy_(torch.tensor([int(step)], dtype=torch.int64).view(torch.int32))
         self.steps = int(step)
 
+    def _set_seed(self, seed):
+        self.seed = int(seed)
+        self._words[5] = ((self.seed & 0xFFFFFFFF) ^ 0x80000000) - 0x80000000          # 32 bits of the seed as an int32
+
+    def reset(self, seed):
+        """as before the first step, in the same memory"""
+        self.exp_avg.zero_()
+        self.exp_avg_sq.zero_()
+        if self.exponents is not None:
+            self.exponents.fill_(1)                        # the smallest exponent, a block of zeros
+        self._set_seed(seed)
+        self.set_step(0)
+
     def state_dict(self):
         """flat states (tensor i at self.offsets[i], sizes[i] elements), on the device; synchronises for the step counter"""
         out = dict(step=self.device_step(), state_bits=self.state_bits, lr=self.param_groups[0]['lr'], seed=self.seed, sizes=list(self.sizes),
@@ -384,8 +397,7 @@ class AdamW:
             dst.copy_(src)
         self.set_step(state['step'])
         if 'seed' in state:
-            self.seed = int(state['seed'])
-            self._words[5] = ((self.seed & 0xFFFFFFFF) ^ 0x80000000) - 0x80000000
+            self._set_seed(state['seed'])
         if 'lr' in state:
             self.param_groups[0]['lr'] = state['lr']
 
@@ -511,7 +523,10 @@ class ClipAdamW:
             if state['state_bits'] != self.state_bits or (held and held[-1] >= len(self.arena.slots)):
                 raise MsclError('ClipAdamW: the state belongs to another model or another state_bits')
             self.param_groups[0]['lr'] = state['lr']
-            if not held:
+            if not held:                                   # from before the first step
+                if self._inner is not None:
+                    self._inner.reset(self._args['seed'])
+                self.steps = 0
                 return
             for i in held:
                 self.arena.slots[i].touched = True         # as at the step that wrote the state

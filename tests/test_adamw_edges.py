@@ -273,3 +273,20 @@ def test_amsgrad_states_are_refused(dev):
     with pytest.raises(NotImplementedError, match='amsgrad'):
         opt.load_state_dict(topt.state_dict())
     assert opt._inner is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+def test_the_state_from_before_the_first_step(bits, dev):
+    """loaded into an optimizer that has stepped, it takes that one back to its beginning"""
+    model, opt = _net(dev, bits)
+    first = opt.state_dict()
+    q = model.arena.Q.clone()
+    _train(model, opt, 2)
+    want = model.arena.Q.clone()
+    opt.load_state_dict(first)
+    assert opt.steps == 0 and opt._inner.device_step() == 0
+    assert not any(v.any() for v in opt._inner.state_values())
+    model.arena.Q.copy_(q)
+    _train(model, opt, 2)
+    assert torch.equal(model.arena.Q, want)
