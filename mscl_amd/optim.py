@@ -192,6 +192,21 @@ def _check_args(lr, betas, eps, weight_decay, grad_clip, state_bits, seed=0):
         raise MsclError('AdamW: grad_clip needs max_norm > 0 (None: no clip)')
 
 
+def _check_state(state, state_bits, sizes):
+    """refuses a state that does not belong to tensors of these sizes"""
+    if state['state_bits'] != state_bits:
+        raise MsclError(f"AdamW: a state of {state['state_bits']} bits does not fit state_bits={state_bits}")
+    if state['step'] < 0:
+        raise MsclError('AdamW: a negative step')
+    total = _layout(sizes)[2]
+    want = dict(exp_avg=(total,), exp_avg_sq=(total,))
+    if state_bits == 8:
+        want['exponents'] = (2, total // BLOCK)
+    if (list(state.get('sizes', sizes)) != list(sizes) or          # (states written without them are told by the total alone)
+            any(tuple(state[k].shape) != shape or state[k].dtype != (torch.float32 if state_bits == 32 else torch.uint8) for k, shape in want.items())):
+        raise MsclError('AdamW: the state belongs to other parameters')
+
+
 _raise_version = getattr(torch._C, '_increment_version', None) or torch.autograd.graph.increment_version          # (raw: 4 / 62 tensors 0.6 / 4.0 us, not 1.2 / 5.6)
 
 
@@ -381,18 +396,10 @@ class AdamW:
         return out
 
     def load_state_dict(self, state):
-        if state['state_bits'] != self.state_bits:
-            raise MsclError(f"AdamW: a state of {state['state_bits']} bits does not fit state_bits={self.state_bits}")
-        if state['step'] < 0:
-            raise MsclError('AdamW: a negative step')
-        if list(state.get('sizes', self.sizes)) != self.sizes:          # (states written without them are told by the total alone)
-            raise MsclError('AdamW: the state belongs to other parameters')
+        _check_state(state, self.state_bits, self.sizes)
         pairs = [(self.exp_avg, state['exp_avg']), (self.exp_avg_sq, state['exp_avg_sq'])]
         if self.state_bits == 8:
             pairs.append((self.exponents, state['exponents']))
-        for dst, src in pairs:
-            if src.shape != dst.shape or src.dtype != dst.dtype:
-                raise MsclError('AdamW: the state belongs to other parameters')
         for dst, src in pairs:
             dst.copy_(src)
         self.set_step(state['step'])
@@ -519,9 +526,13 @@ class ClipAdamW:
         """a state_dict() of this class, or torch.optim.AdamW's own (the reference's checkpoints; 32-bit states only), whose entries are
         keyed by the parameter's index in model.parameters()"""
         if 'slots' in state:
-            held = list(state['slots'])
-            if state['state_bits'] != self.state_bits or (held and held[-1] >= len(self.arena.slots)):
+            held, slots = list(state['slots']), self.arena.slots
+            if state['state_bits'] != self.state_bits or any(not 0 <= i < len(slots) for i in held):
                 raise MsclError('ClipAdamW: the state belongs to another model or another state_bits')
+            if held:                                       # all of it is looked at before anything is changed
+                _check_state(state, self.state_bits, [slots[i].numel for i in held])
+                if held != sorted(set(held) | {i for i, s in enumerate(slots) if s.touched}):
+                    raise MsclError('ClipAdamW: other parameters receive gradients than in the state')
             self.param_groups[0]['lr'] = state['lr']
             if not held:                                   # from before the first step
                 if self._inner is not None:
@@ -529,10 +540,8 @@ class ClipAdamW:
                 self.steps = 0
                 return
             for i in held:
-                self.arena.slots[i].touched = True         # as at the step that wrote the state
+                slots[i].touched = True                    # as at the step that wrote the state
             self._build()
-            if self._slot_indices() != held:
-                raise MsclError('ClipAdamW: other parameters receive gradients than in the state')
             self._inner.load_state_dict(state)
             self.steps = self._inner.steps
             return
@@ -546,7 +555,7 @@ class ClipAdamW:
             if st is None:
                 continue
             slot = getattr(p, '_mscl_slot', None)
-            if slot is None or not p.requires_grad or tuple(st['exp_avg'].shape) != tuple(p.shape):
+            if slot is None or not p.requires_grad or any(tuple(st[k].shape) != tuple(p.shape) for k in ('exp_avg', 'exp_avg_sq')):
                 raise ValueError(f'optimizer state {idx} does not belong to trainable parameter {idx} of this model')
             step = max(step, int(st['step']))
             found.append((slot, st))

@@ -290,3 +290,34 @@ def test_the_state_from_before_the_first_step(bits, dev):
     model.arena.Q.copy_(q)
     _train(model, opt, 2)
     assert torch.equal(model.arena.Q, want)
+
+
+@pytest.mark.gpu
+def test_a_refused_state_changes_nothing(dev):
+    """states of another model, of other parameters or damaged ones: parameters that take part, moments, counter and rate stay"""
+    from mscl_amd.lib import MsclError
+    model, opt = _net(dev)
+    _train(model, opt, 2)
+    whole = opt.state_dict()
+    part, popt = _net(dev)
+    _train(part, popt, 1, upto=2)                          # `last` has received no gradient
+    before = popt.state_dict()
+    inner, slots = popt._inner, list(popt._slots)
+    bad = [dict(whole, slots=[0, 99]), dict(whole, exp_avg=whole['exp_avg'][:256]), dict(whole, exp_avg_sq=whole['exp_avg_sq'].double()),
+           dict(whole, slots=whole['slots'][1:]), dict(whole, step=-1), dict(whole, state_bits=8)]
+    other = _torch_state(part, [1e-3] * len(list(part.parameters())))
+    worse = {k: dict(v) for k, v in other['state'].items()}
+    worse[4] = dict(worse[4], exp_avg_sq=worse[4]['exp_avg_sq'][:3])
+    for state in bad + [dict(other, state=worse)]:
+        with pytest.raises((MsclError, ValueError)):
+            popt.load_state_dict(state)
+        assert popt._inner is inner and popt._slots == slots and [s for s in part.arena.slots if s.touched] == slots
+        after = popt.state_dict()
+        assert all(torch.equal(v, after[k]) if torch.is_tensor(v) else v == after[k] for k, v in before.items()), state.get('slots')
+    for state in bad:                                      # the same before the first step
+        fresh, fopt = _net(dev)
+        with pytest.raises(MsclError):
+            fopt.load_state_dict(state)
+        assert fopt._inner is None and not any(s.touched for s in fresh.arena.slots) and fopt.param_groups[0]['lr'] == 1e-3
+    popt.load_state_dict(whole)                            # a whole one for more parameters is taken: nothing of it is captured
+    assert popt._slot_indices() == whole['slots'] and popt.steps == 2
