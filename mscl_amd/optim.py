@@ -514,6 +514,12 @@ class ClipAdamW:
         if self._inner is not None:
             self._inner.sync_lr()
 
+    def _check_rebuild(self, loaded):
+        """refuses a state whose parameters, beside those that take part by now, need another optimizer while a captured step uses this one"""
+        inner = self._inner
+        if inner is not None and (inner._in_graph or inner._kept) and any(s not in self._slots for s in loaded):
+            raise MsclError('ClipAdamW: the state has parameters that a captured step does not update: load it into an optimizer that is not captured')
+
     def _slot_indices(self):
         return [i for i, s in enumerate(self.arena.slots) if any(s is t for t in self._slots)]
 
@@ -533,6 +539,7 @@ class ClipAdamW:
                 _check_state(state, self.state_bits, [slots[i].numel for i in held])
                 if held != sorted(set(held) | {i for i, s in enumerate(slots) if s.touched}):
                     raise MsclError('ClipAdamW: other parameters receive gradients than in the state')
+                self._check_rebuild([slots[i] for i in held])
             self.param_groups[0]['lr'] = state['lr']
             if not held:                                   # from before the first step
                 if self._inner is not None:
@@ -563,6 +570,7 @@ class ClipAdamW:
             raise MsclError('ClipAdamW: the checkpoint holds no AdamW moments')
         mult = [self._mult.get(getattr(p, '_mscl_slot', None), (1.0, 1.0))[0] if p.requires_grad else 1.0 for p in params]
         lr = _base_lr(state.get('param_groups') or [{}], mult)
+        self._check_rebuild([slot for slot, _ in found])
         for slot, _ in found:
             slot.touched = True
         self._build()

@@ -321,3 +321,33 @@ def test_a_refused_state_changes_nothing(dev):
         assert fopt._inner is None and not any(s.touched for s in fresh.arena.slots) and fopt.param_groups[0]['lr'] == 1e-3
     popt.load_state_dict(whole)                            # a whole one for more parameters is taken: nothing of it is captured
     assert popt._slot_indices() == whole['slots'] and popt.steps == 2
+
+
+@pytest.mark.gpu
+def test_a_captured_step_keeps_its_memory(dev):
+    """a captured step reads and writes the optimizer's buffers: a state that would need others is refused, one that fits goes into them"""
+    from mscl_amd.lib import MsclError
+    model, opt = _net(dev)
+    _train(model, opt, 2)
+    whole = opt.state_dict()
+    part, popt = _net(dev)
+    _train(part, popt, 1, upto=2)
+    own = popt.state_dict()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        popt.step()
+    inner = popt._inner
+    for state in (whole, _torch_state(part, [1e-3] * len(list(part.parameters())))):
+        with pytest.raises(MsclError, match='captured'):
+            popt.load_state_dict(state)
+        assert popt._inner is inner and not all(s.touched for s in part.arena.slots)
+    q = part.arena.Q.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    want = part.arena.Q.clone()
+    popt.load_state_dict(own)
+    part.arena.Q.copy_(q)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(part.arena.Q, want) and popt._inner is inner and inner.device_step() == 2
