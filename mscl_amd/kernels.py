@@ -628,18 +628,21 @@ class ResNormSaved:
 
     def restored(self, x, f, gate, stats):
         """a whole one again from release()'s tensors, which may lie elsewhere and otherwise by now"""
-        s, d = ResNormSaved(), lib.ResNormDesc.from_buffer_copy(self.desc)
-        x, d.ld_x = _rows_of(x, d.C)
+        s, d = ResNormSaved(), self.desc
+        x, ld_x = _rows_of(x, d.C)
+        ld_f = d.ld_f
         if f is not None:
-            f, d.ld_f = _rows_of(f, d.C)
+            f, ld_f = _rows_of(f, d.C)
         if gate is not None:
             gate = gate.contiguous()
         stats = stats.contiguous()
-        d.x, d.f, d.gate = x.data_ptr(), _at(f), _at(gate)
-        for k in ('mean_f', 'rstd_f', 'mean_y', 'rstd_y'):
-            at = getattr(d, k)
-            if at:
-                setattr(d, k, at - self.stats_at + stats.data_ptr())
+        at, to = (d.x, d.f, d.gate, d.ld_x, d.ld_f, self.stats_at), (x.data_ptr() or None, _at(f), _at(gate), ld_x, ld_f, stats.data_ptr())
+        if at != to:
+            d = lib.ResNormDesc.from_buffer_copy(d)
+            d.x, d.f, d.gate, d.ld_x, d.ld_f = to[:5]
+            for k in ('mean_f', 'rstd_f', 'mean_y', 'rstd_y'):
+                if getattr(d, k):
+                    setattr(d, k, getattr(d, k) - self.stats_at + to[5])
         s.x, s.f, s.gate, s.stats, s.stats_at, s.desc = x, f, gate, stats, stats.data_ptr(), d
         s.vec, s.names, s.shape, s.kind = self.vec, self.names, self.shape, self.kind
         return s

@@ -1029,7 +1029,7 @@ class ResNormHip(nn.Module):
                     b_pre=0.0 if pre and bias else None)
         for name, v in fill.items():
             self.register_parameter(name, None if v is None else nn.Parameter(torch.full((channels,), float(v))))
-        self._rt = None
+        self._rt = self._anchor = None
 
     def extra_repr(self):
         return f'{self.channels}, post={self.post}, pre={self.pre}, gate_act={self.gate_act}, eps={self.eps}'
@@ -1044,6 +1044,15 @@ class ResNormHip(nn.Module):
         """the parameters that a backward pass reaches"""
         return [k for k in self._rt['slots'] if (dh if k.endswith('pre') else branch)]
 
+    def _leaf(self, device):
+        # The calls of a capture have one each: a shared leaf has one accumulation node, which stays on the stream of its first call, and a
+        # capture that meets it while an eager graph lives waits on that stream.
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(0, device=device, requires_grad=True)
+        if self._anchor is None or self._anchor.device != device:
+            self._anchor = torch.empty(0, device=device, requires_grad=True)
+        return self._anchor
+
     def forward(self, x, f=None, gate=None):
         """(y, h); without a branch f the input norm of a first block: (x, norm_pre(x))"""
         if self._rt is None:
@@ -1053,10 +1062,8 @@ class ResNormHip(nn.Module):
             return y, h
         # copies that the kernels need (gaps between rows that no stride describes) are made here, in autograd's sight
         x, f = (t if t is None or t.is_contiguous() else K._rows_of(t, t.shape[-1])[0] for t in (x, f))
-        # The parameters' gradients need the node also where no input does.  A leaf of the call's own: one that calls share has one accumulation
-        # node, which stays on the stream of the first call, and a capture that meets it while an eager graph lives waits on that stream.
         anchor = None
-        if not any(t is not None and t.requires_grad for t in (x, f, gate)):
-            anchor = torch.empty(0, device=x.device, requires_grad=True)
+        if not any(t is not None and t.requires_grad for t in (x, f, gate)):          # the parameters' gradients need the node all the same
+            anchor = self._leaf(x.device)
         out = _ResNormFn.apply(x, f, gate if gate is None else gate.contiguous(), anchor, self)
         return (x, out) if f is None else out if self.pre is not None else (out, None)
