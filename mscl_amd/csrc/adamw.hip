@@ -16,8 +16,8 @@
 // What bounds it (MI355X, where a copy of 4 GB runs at 4.8 TB/s and an in-place add at 5.9): memory.  Counters give the bytes of the
 // formula and no more: 26 per element for 16-bit gradients and no shadow, 320 M elements in 1.48 ms = 5.6 TB/s; 33 M elements with fp32
 // gradients, a clip and a shadow (30 bytes, 4 more where the gradient is read a second time, partly from the last-level cache): 25 us for the
-// norm, 5 for the coefficient, 151 for the update.  8 bits: 16 bytes per element, 300 M in 0.85 ms = 5.7 TB/s with the vector units busy
-// about four fifths of the time (78 instructions per element, two of them quarter-rate multiplies of the hash).
+// norm, 5 for the coefficient, 150 for the update.  8 bits: 16 bytes per element, 300 M in 0.85 ms = 5.7 TB/s with the vector units busy
+// about four fifths of the time (80 instructions per element, two of them quarter-rate multiplies of the hash).
 #include "common.h"
 #include <hip/hip_fp16.h>
 #include <cfloat>

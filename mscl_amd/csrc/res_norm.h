@@ -18,7 +18,8 @@
 // Accesses are 16 bytes at the alignment of an element (the memory path of gfx950 takes any), so odd widths and strides run the same
 // code.
 //
-// What bounds it (a copy of 4 GB: 4.8 TB/s, 256 MB: 5.4): memory.  Counters give the bytes of the formula and no more.  Forward, 32768 x 2048,
+// What bounds it (a copy of 4 GB: 4.8 TB/s, 256 MB: 5.4): memory.  Counters give the bytes of the formula, for a backward pass the
+// blocks' column sums besides (16384 x 4096: 8 MB of 1.49 GB).  Forward, 32768 x 2048,
 // fp32 residual and bf16 branch, 805 MB: 146 us, 5.5 TB/s; 401408 x 64 bf16: 41 us, 5.0.  Backward, 401408 x 64: 308 MB in 64 us, 4.8 TB/s;
 // 16384 x 4096, fp32 / bf16, a gate per element: 1.48 GB in 304 us, 4.9 TB/s.  The second launch of a backward pass: 6 - 20 us.
 #include "common.h"

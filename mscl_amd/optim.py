@@ -222,7 +222,8 @@ class AdamW:
 
     `step(grads)` takes one gradient per parameter -- fp32, bf16 or fp16, one type for all, laid out like the parameter -- or reads
     `p.grad`; a parameter whose gradient is None is refused (build the optimizer over the parameters that train).  lr is
-    `param_groups[0]['lr']`, read from a device word: set it between steps, and call sync_lr() before replaying a captured step.  The
+    `param_groups[0]['lr']`, read from a device word: set it between steps, and call sync_lr() before replaying a captured step (betas, eps >=
+    2^-126 and weight_decay are fixed: a change of them is refused).  The
     step counter lives on the device, so a captured step counts its replays; capture a step only after an eager one with the same
     gradient tensors (their addresses are uploaded by the eager one)."""
 
@@ -530,7 +531,8 @@ class ClipAdamW:
 
     def load_state_dict(self, state):
         """a state_dict() of this class, or torch.optim.AdamW's own (the reference's checkpoints; 32-bit states only), whose entries are
-        keyed by the parameter's index in model.parameters()"""
+        keyed by the parameter's index in model.parameters() and whose groups hold lr times the parameter's multiplier (one step counter: the
+        largest of the entries').  A state that is refused changes nothing"""
         if 'slots' in state:
             held, slots = list(state['slots']), self.arena.slots
             if state['state_bits'] != self.state_bits or any(not 0 <= i < len(slots) for i in held):

@@ -4,10 +4,13 @@ Tolerances, with u = 2^-24 (a rounding of fp32): a result is off by one rounding
 bf16, fp16 (1/2 of eps; 2^-24 for fp32) -- plus K u times the magnitude that the oracle gives beside it (the formula with every term
 positive).  K counts fp32 roundings on the longest path: a row sum is 16 values in a lane, up to 10 steps in a wave and 16 over the
 waves (42), then mean, + eps, square root, division (4): 1 / deviation is good to 46 u / 2 + 4, a normalised value to ~30 u and 4 more for
-the mean of a layer norm (42 again): n 80 u;  w, b, scale, act (expf and tanhf: 2 ulp each, division 1), add: y 90 u;  the second norm on top: yhat 90 + 80,
-h 175 u;  its backward: product, row sum, 3 more: dx 175 + 50 = 225 u;  the branch's: 225 + 5 + 50 + 80: df 360 u;  column sums: 230 + 80 per term and one
-rounding per row in a thread and 32 rows in a block (the second launch adds in 64 bits): 310 + rows_in_a_thread + 32.  K = 512 covers all of them
-while a thread adds up to 128 rows; the tests stay below (at most 6000 rows over teams of 16 .. 1024 lanes, 1024 blocks or fewer rows)."""
+the mean of a layer norm (42 again): n 80 u;  w, b, scale, act (the kernels' exponential 2 ulp, 1 + e, the 1-ulp reciprocal and a product: 8 u;
+tanhf 2 ulp), add: y 95 u;  the second norm on top: yhat 95 + 80, h 180 u;  its backward: product, row sum, 3 more: dx 180 + 50 = 230 u;  the
+branch's: 230 + 5 + 50 + 80: df 365 u;  column sums: 230 + 90 per term (90: n and a gate's value or slope), one rounding per row in a thread and one
+for each of a block's 256 / T teams of T lanes (the second launch adds in 64 bits): 320 + rows_in_a_thread + 32 for T >= 8.  Up to 32 channels T is
+1 .. 4, with up to 256 teams, but a row sum is 8 values and 2 steps: n 20 u, y 35, yhat 60, dx 85, a column's term 125: 125 + rows_in_a_thread + 256.
+K = 512 covers all of them while a thread adds up to 128 rows; the tests stay below (at most 6000 rows over teams of 16 .. 1024 lanes, 1024 blocks
+or fewer rows)."""
 import itertools
 import random
 
