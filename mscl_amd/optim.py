@@ -438,12 +438,15 @@ def _base_lr(groups, mult):
     parameter, lr times its multiplier); None where no group tells.  mult: lr multiplier of each parameter index"""
     if any(not 0 <= i < len(mult) for g in groups for i in g.get('params', ())):
         raise MsclError("ClipAdamW: the state's groups hold parameters that the model has not")
-    rates = [float(g['lr']) / mult[i] for g in groups if 'lr' in g for i in g.get('params', ()) if mult[i] > 0]
-    if not rates:
+    known = [(i, g) for g in groups if 'lr' in g for i in g.get('params', ()) if mult[i] > 0]
+    if not known:
         return float(groups[0]['lr']) if 'lr' in groups[0] and 'params' not in groups[0] else None
+    key = 'initial_lr' if all('initial_lr' in g for _, g in known) else 'lr'          # a schedule's floor is the same for all groups
+    rates = [float(g[key]) / mult[i] for i, g in known]
     if max(rates) - min(rates) > 1e-6 * max(rates):
         raise MsclError(f'ClipAdamW: the state holds rates from {min(rates)} to {max(rates)} without their lr_mult: built with another paramwise_cfg')
-    return rates[0]
+    i, g = min(known, key=lambda e: abs(mult[e[0]] - 1))
+    return float(g['lr']) / mult[i]
 
 
 class ClipAdamW:

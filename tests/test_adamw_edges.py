@@ -351,3 +351,25 @@ def test_a_captured_step_keeps_its_memory(dev):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(part.arena.Q, want) and popt._inner is inner and inner.device_step() == 2
+
+
+def test_rates_of_a_schedule_with_a_floor():
+    """mmcv's schedules start from initial_lr and may end at one min_lr for all groups: their rates then differ by more than the multipliers, but
+    the groups agree on where they started, and one without a multiplier tells the rate"""
+    from mscl_amd.lib import MsclError
+    from mscl_amd.optim import _base_lr
+    mult, low, c = [0.1, 1.0, 0.0, 10.0], 1e-5, 0.3
+
+    def groups(start):
+        return [dict(params=[i], initial_lr=s, lr=low + (s - low) * c) for i, s in enumerate(start)]
+    assert abs(_base_lr(groups([2e-3 * m for m in mult]), mult) / (low + (2e-3 - low) * c) - 1) < 1e-12
+    with pytest.raises(MsclError, match='rate'):
+        _base_lr(groups([2e-3] * 4), mult)
+    half = groups([2e-3 * m for m in mult])
+    del half[1]['initial_lr']
+    with pytest.raises(MsclError, match='rate'):
+        _base_lr(half, mult)
+    assert _base_lr([dict(params=[0, 1, 2, 3], lr=3e-4)], [1.0] * 4) == 3e-4
+    assert _base_lr([dict(lr=3e-4)], mult) == 3e-4 and _base_lr([{}], mult) is None and _base_lr([dict(params=[2], lr=0.0)], mult) is None
+    with pytest.raises(MsclError, match='has not'):
+        _base_lr([dict(params=[4], lr=1.0)], mult)
