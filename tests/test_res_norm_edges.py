@@ -214,3 +214,46 @@ def test_captured_beside_a_living_eager_graph(dev):
     first = ar.G.clone()
     torch.autograd.backward([keep], [torch.zeros_like(dy)])          # the eager graph is still whole
     assert torch.equal(first, ar.G)
+
+
+@pytest.mark.gpu
+def test_recomputed_in_a_checkpoint(dev):
+    """activation checkpointing throws the saved tensors away and makes them again: the same gradients, added to the arena once"""
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(1)
+    x0, f0, gate, dy = torch.randn(40, 16, device=dev), torch.randn(40, 16, device=dev), torch.randn(4, 16, device=dev), torch.randn(40, 16, device=dev)
+    want = None
+    for recompute in (False, True):
+        m, ar = _module(dev)
+        x, f = x0.clone().requires_grad_(), f0.clone().requires_grad_()
+
+        def block(a, b):
+            y, h = m(a * 2.0, b, gate)
+            return y + h.tanh()
+        out = checkpoint(block, x, f, use_reentrant=False) if recompute else block(x, f)
+        out.backward(dy)
+        got = [x.grad.clone(), f.grad.clone(), ar.G.clone()]
+        assert want is None or all(torch.equal(a, b) for a, b in zip(want, got))
+        want = got
+
+
+@pytest.mark.gpu
+def test_inputs_of_any_layout(dev):
+    """permuted, strided and broadcast inputs of the module against dense copies of them: outputs and gradients, bit for bit"""
+    torch.manual_seed(2)
+    base = torch.randn(3, 16, 5, 4, device=dev)
+    forms = dict(permuted=lambda t: t.permute(0, 2, 3, 1), part=lambda t: t.permute(0, 2, 3, 1)[:, 1:4], row=lambda t: t[:, :, :1, :1].permute(0, 2, 3, 1),
+                 spread=lambda t: t[:1, :, :1].permute(0, 2, 3, 1).expand(3, 5, 4, 16))
+    for name, form in forms.items():
+        got = []
+        for dense in (False, True):
+            m, ar = _module(dev)
+            x, f, gate = base.clone().requires_grad_(), (base * 0.5 + 1).requires_grad_(), torch.linspace(-2, 2, 48, device=dev).view(16, 3).requires_grad_()
+            a, b, c = form(x), form(f), gate.t()
+            y, h = m(*(t.contiguous() for t in (a, b, c))) if dense else m(a, b, c)
+            gx, gf, gg = torch.autograd.grad((y * 1.5).sum() + (h * h).sum(), [x, f, gate], create_graph=True)
+            assert gx.shape == x.shape and gg.shape == gate.shape
+            with pytest.raises(RuntimeError, match='once_differentiable'):
+                torch.autograd.grad(gx.square().sum() + x.sum(), x)
+            got.append([y.detach().clone(), h.detach().clone(), gx.detach(), gf.detach(), gg.detach(), ar.G.clone()])
+        assert all(torch.equal(p, q) for p, q in zip(*got)), name
